@@ -601,6 +601,54 @@ int lr_jacobi_det_stats_f32(const float* map, int B, int D, int W, int H, float 
                             double* partial, int nblk, double* out, void* stream);
 
 /* ------------------------------------------------------------------------
+ * Layer norm over the last axis of a dense (rows, cols) array, LeakyReLU in the same pass, and its gradient: the normalisation
+ * of the conv blocks (channels-last activations: a row is a voxel's channels) and of the FC head in place of the batch norm that
+ * the reference's convBlock offers (src/liftreg/layers/layers.py:335-372) and a batch of 1-8 volumes cannot feed.
+ *     xhat = (x - mean) / sqrt(var + eps),  z = xhat w + b,  y = z >= 0 ? z : slope z        (var: of the row, divided by cols)
+ *     g = gy (z >= 0 ? 1 : slope),  h = g w,  gx = (h - mean(h) - xhat mean(h xhat)) / sqrt(var + eps)
+ *     gw = sum over rows of g xhat,  gb = sum over rows of g
+ * x, y, gy, gx: dev, fp32 or (bf16 != 0) bfloat16, any alignment of their elements; w, b (cols): dev fp32, nullable (1 and 0);
+ * gx, gw, gb nullable (not computed).  Sums in fp32, fixed order.  rows >= 0, cols >= 1.
+ * stats: dev fp32 (rows, 2), mean and 1 / sqrt(var + eps).  lr_layer_norm writes it if it is not NULL.  lr_layer_norm_bwd reads
+ *   it if it is not NULL (and rows are longer than lr_layer_norm_resident_cols(): shorter ones are held in registers, where
+ *   recomputing the statistics costs less than reading them).
+ * workspace: dev, lr_layer_norm_workspace(rows, cols, backward) bytes, 16-byte aligned; NULL if that is 0. */
+int64_t lr_layer_norm_resident_cols(void);
+int64_t lr_layer_norm_workspace(int64_t rows, int64_t cols, int backward);
+int lr_layer_norm(const void* x, const float* w, const float* b, void* y, float* stats, void* workspace, int64_t rows,
+                  int64_t cols, int bf16, float eps, float slope, void* stream);
+int lr_layer_norm_bwd(const void* x, const float* w, const float* b, const void* gy, const float* stats, void* gx, float* gw,
+                      float* gb, void* workspace, int64_t rows, int64_t cols, int bf16, float eps, float slope, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The update of the parameters (the reference: torch.optim.Adam, src/liftreg/networks/RegistrationNet.py:245).
+ *
+ * lr_adamw_step: one AdamW step over n tensors, in place; 64 tensors (56 with 8-bit states) a launch:
+ *     g = grad c;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2
+ *     p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ * params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel: HOST arrays of n entries, read before the call
+ *   returns; the entries are dev pointers to dense tensors of numel[i] elements (0 elements: the entry is skipped).  No two
+ *   written tensors may overlap.  Alignment: the element's.
+ * bf16: params and grads are bfloat16 (rounded to nearest even), else fp32.
+ * exp_avg_scale == exp_avg_sq_scale == NULL: m, v are fp32.  Otherwise 8-bit states: 32 consecutive elements of a tensor share
+ *   one byte s of exp_avg_scale[i] / exp_avg_sq_scale[i] ((numel[i]+31)/32 bytes each): value = code 2^(s-127) (s = 255: NaN),
+ *   codes e4m3 (m) and e5m2 (v), one byte an element, stochastically rounded with bits hashed from (seed, t, position of the
+ *   element in the concatenation of the call's tensors, each padded to whole blocks of 32, mod 2^32).
+ * t = step (>= 1), or *step_dev (dev int64, >= 1) if step_dev is not NULL; lr, or *lr_dev (dev fp32) if lr_dev is not NULL:
+ *   what a captured graph replays with new values.
+ * c = 1, or min(1, max_norm / (norm + 1e-6)) with norm = *norm_in (dev) if norm_in is given, or, if partial (dev workspace of
+ *   lr_grad_norm_partials(numel, n) doubles) is given, the 2-norm of this call's gradients, which is also written to norm_out
+ *   (dev, nullable).  norm_in and partial exclude each other.
+ * lr_grad_norm: norm (dev fp32) = sqrt(sum of squares over n tensors), fp64 sums in a fixed order. */
+int64_t lr_grad_norm_partials(const int64_t* numel, int n);
+int lr_grad_norm(const void* const* grads, const int64_t* numel, int n, int bf16, double* partial, float* norm, void* stream);
+int lr_adamw_step(void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+                  void* const* exp_avg_scale, void* const* exp_avg_sq_scale, const int64_t* numel, int n, int bf16,
+                  double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                  const float* lr_dev, const int64_t* step_dev, float max_norm, const float* norm_in, double* partial,
+                  float* norm_out, uint64_t seed, void* stream);
+
+/* ------------------------------------------------------------------------
  * EXPERIMENTAL — not part of the product build.  `make -C liftreg_amd/csrc exp` compiles the library with -DLR_EXPERIMENTAL
  * (plus conv0_pc.hip) into libliftreg_hip_exp.so; LIFTREG_HIP_LIB=<that file> makes liftreg_amd load it (tests of these paths
  * skip on the product library).  Both paths are bit-tested against the default ones and were measured no faster:

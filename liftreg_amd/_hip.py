@@ -23,7 +23,7 @@ NCC_CONFIGURED, NCC_SQUARED = 0, 1
 MAX_VIEWS = 32
 
 _p = C.c_void_p
-_i, _i64, _f = C.c_int, C.c_int64, C.c_float
+_i, _i64, _f, _d = C.c_int, C.c_int64, C.c_float, C.c_double
 
 # name -> (restype, argtypes); mirrors include/liftreg_hip.h one to one
 SIGNATURES = {
@@ -97,6 +97,13 @@ SIGNATURES = {
     "lr_normalize_clip_f32": (_i, [_p, _p, _i64, _f, _f, _p]),
     "lr_label_overlap_f32": (_i, [_p, _p, _f, _i64, _p, _i, _p, _p]),
     "lr_jacobi_det_stats_f32": (_i, [_p, _i, _i, _i, _i, _f, _f, _f, _p, _i, _p, _p]),
+    "lr_layer_norm_resident_cols": (_i64, []),
+    "lr_layer_norm_workspace": (_i64, [_i64, _i64, _i]),
+    "lr_layer_norm": (_i, [_p] * 6 + [_i64, _i64, _i, _f, _f, _p]),
+    "lr_layer_norm_bwd": (_i, [_p] * 9 + [_i64, _i64, _i, _f, _f, _p]),
+    "lr_grad_norm_partials": (_i64, [_p, _i]),
+    "lr_grad_norm": (_i, [_p, _p, _i, _i, _p, _p, _p]),
+    "lr_adamw_step": (_i, [_p] * 7 + [_i, _i, _d, _d, _d, _d, _d, _i64, _p, _p, _f, _p, _p, _p, C.c_uint64, _p]),
     "lr_conv3d_wgrad_partial_floats": (_i64, [_i, _i, _i, _i]),
     "lr_conv3d_wgrad_f32": (_i, [_p, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p]),
 }

@@ -173,6 +173,28 @@ class LinearFn(torch.autograd.Function):
         return gx, gw, (gb if has_bias else None), None
 
 
+class LayerNormFn(torch.autograd.Function):
+    """LeakyReLU(layer norm over the last axis).  `premasked_grad`: the gradient that arrives has gone through the LeakyReLU's mask
+    (a conv block that consumes the output applies it in its data gradient, see ConvBlockFn's mask_input_slope)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, slope, premasked_grad=False):
+        y, stats = ops.layer_norm(x, weight, bias, eps=eps, negative_slope=slope, return_stats=True)
+        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.cfg = (eps, 1.0 if premasked_grad else slope)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, stats = ctx.saved_tensors
+        eps, slope = ctx.cfg
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        gx, gw, gb = ops_bwd.layer_norm_bwd(x, weight, bias, gy, eps=eps, negative_slope=slope, stats=stats, need_gx=need_x,
+                                            need_gwb=need_w or need_b)
+        return gx, gw if need_w else None, gb if need_b else None, None, None, None
+
+
 class PCAFn(torch.autograd.Function):
     """disp = coefs @ basis + mean; only the coefficients receive a gradient (the basis is data)."""
 

@@ -1,0 +1,701 @@
+// layernorm.hip — layer norm over the last axis, LeakyReLU in the same pass, and its gradient with the reduction of the weight's.
+//
+//   xhat = (x - mean) rstd,  z = xhat w + b,  y = z >= 0 ? z : slope z
+//   g = gy (z >= 0 ? 1 : slope),  h = g w,  gx = rstd (h - mean(h) - xhat mean(h xhat))
+//   gw[c] = sum over rows of g xhat,  gb[c] = sum over rows of g
+//
+// Bound by memory: x and y once forward; x, gy and gx once backward.  Two forms, by the length of a row:
+//  * up to kResident columns a row lives in the registers of a group of G lanes (a quarter of a wave for the 16 channels of a voxel,
+//    a wave for the head's 800 features, a workgroup above 1024 columns), 16 bytes a lane and load.  Mean and variance are two
+//    passes over registers.  Backward recomputes them: x is there anyway, and 8 bytes of saved statistics a row would be 1/8 of a
+//    16-channel row forward and again backward.  A lane keeps its columns over all its rows, so the weight's gradient grows in
+//    registers; groups, then waves add theirs, each workgroup leaves one partial row, a second kernel adds those in a fixed order.
+//  * longer rows are cut into chunks (few rows would leave most CUs idle): per-chunk mean and M2 (Chan's update), joined per row,
+//    then one pass that normalises; backward the same with the sums of h and h xhat, where a workgroup of the last pass owns columns
+//    and walks down the rows, so the weight's gradient needs no atomics either.
+#include "lr_common.h"
+
+namespace {
+
+constexpr int kResident = 16384;       // longest row that is held in registers: 1024 lanes of 16 elements
+constexpr int kBlocks = 2048;          // workgroups of the resident kernels: eight of four waves on each of 256 CUs
+constexpr int kFinish = 32;            // columns of a workgroup that adds partial rows
+
+template <class T> struct Vec;
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+template <> struct Vec<uint16_t> {     // bfloat16
+  static constexpr int N = 8;
+  typedef uint16_t V __attribute__((ext_vector_type(8), aligned(2)));
+  static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+  static __device__ __forceinline__ uint16_t down(float v) {   // nearest even; NaN stays NaN
+    const uint32_t u = __float_as_uint(v);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+  }
+};
+
+// N elements from column c of a row of C (past the end: 0, not written).  A row may start at any element: gfx950 takes 16-byte
+// accesses at any address.
+template <class T>
+__device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* r) {
+  constexpr int N = Vec<T>::N;
+  if (c + N <= C) {
+    const typename Vec<T>::V v = *reinterpret_cast<const typename Vec<T>::V*>(row + c);
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = Vec<T>::up(v[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = c + e < C ? Vec<T>::up(row[c + e]) : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float* r) {
+  constexpr int N = Vec<T>::N;
+  if (c + N <= C) {
+    typename Vec<T>::V v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = Vec<T>::down(r[e]);
+    *reinterpret_cast<typename Vec<T>::V*>(row + c) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < C) row[c + e] = Vec<T>::down(r[e]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_f(const float* a, int64_t c, int64_t C, float other, float* r) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) r[e] = other;
+  if (!a) return;
+  if (c + N <= C) {
+#pragma unroll
+    for (int q = 0; q < N; q += 4) load(a, c + q, C, r + q);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (c + e < C) r[e] = a[c + e];
+  }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float x) {
+  return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// sum over aligned groups of G lanes, in every lane
+template <int G>
+__device__ __forceinline__ float lane_sum(float x) {
+  if (G >= 2) x = add_dpp<0xB1>(x);      // neighbour
+  if (G >= 4) x = add_dpp<0x4E>(x);      // pair
+  if (G >= 8) x = add_dpp<0x141>(x);     // mirrored half row of 8
+  if (G >= 16) x = add_dpp<0x140>(x);    // mirrored row of 16
+  if (G >= 32) x += __shfl_xor(x, 16, 64);
+  if (G >= 64) x += __shfl_xor(x, 32, 64);
+  return x;
+}
+
+// sums over the G lanes of a row.  Above a wave: through LDS, two buffers in turn, one barrier a sum.
+template <int G, int NT>
+struct Group {
+  float (*red)[NT / 64];
+  int turn;
+  __device__ __forceinline__ explicit Group(float (*r)[NT / 64]) : red(r), turn(0) {}
+  __device__ __forceinline__ float sum(float x) {
+    if (G <= 64) return lane_sum<G>(x);
+    x = lane_sum<64>(x);
+    float* buf = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = x;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) s += buf[w];
+    return s;
+  }
+  __device__ __forceinline__ void sum2(float& a, float& b) {
+    a = sum(a);
+    b = sum(b);
+  }
+};
+
+// mean and rstd of a row held as x[K * N]; RAGGED: cols is no multiple of N
+template <int K, int N, int G, bool RAGGED, class Gr>
+__device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int C, float inv, float eps, float& mean, float& rstd) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < K * N; ++i) s += x[i];
+  s = gr.sum(s);
+  mean = s * inv;
+  mean = fmaf(fmaf(-mean, (float)C, s), inv, mean);   // s / C rounded: a constant row has its own value as mean
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * G + lane) * N;
+    float t = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = x[k * N + e] - mean;
+      t = fmaf(d, (!RAGGED || c + e < C) ? d : 0.f, t);
+    }
+    q += RAGGED || c < C ? t : 0.f;
+  }
+  rstd = __builtin_amdgcn_rsqf(fmaf(gr.sum(q), inv, eps));
+}
+
+template <class T, int G, int K, int NT, bool RAGGED>
+__global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                 T* __restrict__ y, float* __restrict__ stats, int64_t rows, int C, float inv,
+                                                 float eps, float slope) {
+  constexpr int N = Vec<T>::N, RPB = NT / G;
+  __shared__ float red[2][NT / 64];
+  Group<G, NT> gr(red);
+  const int lane = threadIdx.x % G;
+  float wv[K * N], bv[K * N];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load_f<N>(w, (k * G + lane) * N, C, 1.f, wv + k * N);
+    load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + k * N);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + threadIdx.x / G;
+    const int cols = r < rows ? C : 0;      // all lanes stay for the sums
+    const T* xr = x + r * C;
+    float v[K * N];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load(xr, (k * G + lane) * N, cols, v + k * N);
+    float mean, rstd;
+    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float z = fmaf((v[k * N + e] - mean) * rstd, wv[k * N + e], bv[k * N + e]);
+        v[k * N + e] = z >= 0.f ? z : z * slope;
+      }
+      store(y + r * C, (k * G + lane) * N, cols, v + k * N);
+    }
+    if (stats && lane == 0 && r < rows) {
+      stats[2 * r] = mean;
+      stats[2 * r + 1] = rstd;
+    }
+  }
+}
+
+// gx (if set) and, where `part` is set, this workgroup's sums of g xhat and g in part[blockIdx.x][2][C]
+template <class T, int G, int K, int NT, bool RAGGED>
+__global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                 const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ part, int64_t rows,
+                                                 int C, float inv, float eps, float slope) {
+  constexpr int N = Vec<T>::N, RPB = NT / G, E = K * N;
+  __shared__ float red[2][NT / 64];
+  Group<G, NT> gr(red);
+  const int lane = threadIdx.x % G;
+  float wv[E], bv[E], aw[E], ab[E];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    load_f<N>(w, (k * G + lane) * N, C, 1.f, wv + k * N);
+    load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + k * N);
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t r = r0 + threadIdx.x / G;
+    const int cols = r < rows ? C : 0;
+    float v[E], g[E];
+#pragma unroll
+    for (int k = 0; k < K; ++k) load(x + r * C, (k * G + lane) * N, cols, v + k * N);
+#pragma unroll
+    for (int k = 0; k < K; ++k) load(gy + r * C, (k * G + lane) * N, cols, g + k * N);
+    float mean, rstd;
+    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
+    if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {     // past the end g = 0: nothing is added
+      const float xh = (v[i] - mean) * rstd;
+      const float gg = fmaf(xh, wv[i], bv[i]) >= 0.f ? g[i] : g[i] * slope;
+      aw[i] = fmaf(gg, xh, aw[i]);
+      ab[i] += gg;
+      const float h = gg * wv[i];
+      s1 += h;
+      s2 = fmaf(h, xh, s2);
+      v[i] = xh;
+      g[i] = h;
+    }
+    gr.sum2(s1, s2);
+    if (gx) {
+      s1 *= inv;
+      s2 *= inv;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const int i = k * N + e;
+          v[i] = rstd * (g[i] - fmaf(v[i], s2, s1));
+        }
+        store(gx + r * C, (k * G + lane) * N, cols, v + k * N);
+      }
+    }
+  }
+  if (!part) return;
+  // groups of a wave, then waves
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    for (int o = G; o < 64; o *= 2) {
+      aw[i] += __shfl_xor(aw[i], o, 64);
+      ab[i] += __shfl_xor(ab[i], o, 64);
+    }
+  float* p = part + (int64_t)blockIdx.x * 2 * C;
+  if (G > 64) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int c = (k * G + lane) * N + e;
+        if (c < C) {
+          p[c] = aw[k * N + e];
+          p[C + c] = ab[k * N + e];
+        }
+      }
+    return;
+  }
+  constexpr int W = G > 64 ? 1 : NT / 64, L = G > 64 ? 1 : G * E;      // waves, columns
+  __shared__ float cols[W][2][L];
+  const int wave = threadIdx.x >> 6, at = threadIdx.x & 63;
+  if (at < G) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        cols[wave % W][0][((k * G + at) * N + e) % L] = aw[k * N + e];
+        cols[wave % W][1][((k * G + at) * N + e) % L] = ab[k * N + e];
+      }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * C; i += NT) {
+    const int which = i >= C, c = i - which * C;
+    float s = 0.f;
+    for (int q = 0; q < W; ++q) s += cols[q][which][c];
+    p[i] = s;
+  }
+}
+
+// out[0..C) = sum of the first half of the partial rows [n][2 C], out2 of the second, in a fixed order
+__global__ __launch_bounds__(1024) void finish_kernel(const float* __restrict__ part, int n, int64_t C, float* __restrict__ gw,
+                                                      float* __restrict__ gb) {
+  __shared__ float red[1024 / kFinish][kFinish + 1];
+  const int64_t c = (int64_t)blockIdx.x * kFinish + threadIdx.x % kFinish;
+  const int j = threadIdx.x / kFinish;
+  float s = 0.f;
+  if (c < 2 * C)
+#pragma unroll 8
+    for (int i = j; i < n; i += 1024 / kFinish) s += part[(int64_t)i * 2 * C + c];
+  red[j][threadIdx.x % kFinish] = s;
+  __syncthreads();
+  for (int o = 1024 / kFinish / 2; o > 0; o >>= 1) {
+    if (j < o) red[j][threadIdx.x % kFinish] += red[j + o][threadIdx.x % kFinish];
+    __syncthreads();
+  }
+  if (j == 0 && c < 2 * C) {
+    float* out = c < C ? gw : gb;
+    if (out) out[c < C ? c : c - C] = red[0][threadIdx.x];
+  }
+}
+
+// ---------------------------------------------------------------- rows that are cut into chunks
+struct Part { float n, mean, m2; };
+__device__ __forceinline__ Part join(Part a, Part b) {   // Chan: exact up to rounding whatever the two sides hold
+  Part r;
+  r.n = a.n + b.n;
+  const float d = b.mean - a.mean, f = r.n > 0.f ? b.n / r.n : 0.f;
+  r.mean = fmaf(d, f, a.mean);
+  r.m2 = a.m2 + b.m2 + d * d * a.n * f;
+  return r;
+}
+__device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in thread 0
+  __shared__ Part red[4];
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    Part q = {__shfl_xor(p.n, o, 64), __shfl_xor(p.mean, o, 64), __shfl_xor(p.m2, o, 64)};
+    p = join(p, q);
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = p;
+  __syncthreads();
+  return join(join(red[0], red[1]), join(red[2], red[3]));
+}
+
+// mean and M2 of chunk blockIdx.x (`len` columns) of row blockIdx.y
+template <class T>
+__global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ x, float* __restrict__ part, int64_t C, int64_t len,
+                                                          int64_t row0) {
+  constexpr int N = Vec<T>::N, K = 16 / N;
+  const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
+  const T* xr = x + row * C;
+  Part p = {0.f, 0.f, 0.f};
+  for (int64_t at = lo; at < hi; at += 256 * 16) {
+    float v[16];
+    int have = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t c = at + (k * 256 + threadIdx.x) * N;
+      load(xr, c, hi, v + k * N);
+      have += (int)max((int64_t)0, min((int64_t)N, hi - c));
+    }
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += v[i];
+    Part t;
+    t.n = (float)have;
+    t.mean = have ? s / t.n : 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float d = at + (k * 256 + threadIdx.x) * N + e < hi ? v[k * N + e] - t.mean : 0.f;
+        q = fmaf(d, d, q);
+      }
+    t.m2 = q;
+    p = join(p, t);
+  }
+  p = block_join(p);
+  if (threadIdx.x == 0) {
+    float* o = part + (row * gridDim.x + blockIdx.x) * 2;
+    o[0] = p.mean;
+    o[1] = p.m2;
+  }
+}
+
+// stats[row] from the row's chunks
+__global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ part, int chunks, int64_t C, int64_t len,
+                                                         float eps, float* __restrict__ stats, int64_t row0) {
+  const int64_t row = row0 + blockIdx.x;
+  Part p = {0.f, 0.f, 0.f};
+  for (int i = threadIdx.x; i < chunks; i += 256) {
+    const float* o = part + (row * chunks + i) * 2;
+    p = join(p, {(float)min(len, C - i * len), o[0], o[1]});
+  }
+  p = block_join(p);
+  if (threadIdx.x == 0) {
+    stats[2 * row] = p.mean;
+    stats[2 * row + 1] = 1.0f / sqrtf(p.m2 / (float)C + eps);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                        T* __restrict__ y, const float* __restrict__ stats, int64_t C, int64_t len,
+                                                        float slope, int64_t row0) {
+  constexpr int N = Vec<T>::N;
+  const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
+  const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+#pragma unroll 4
+  for (int64_t c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
+    float v[N], wv[N], bv[N];
+    load(x + row * C, c, hi, v);
+    load_f<N>(w, c, hi, 1.f, wv);
+    load_f<N>(b, c, hi, 0.f, bv);
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float z = fmaf((v[e] - mean) * rstd, wv[e], bv[e]);
+      v[e] = z >= 0.f ? z : z * slope;
+    }
+    store(y + row * C, c, hi, v);
+  }
+}
+
+// sums of h and h xhat over a chunk of a row
+template <class T>
+__global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                         const T* __restrict__ gy, const float* __restrict__ stats,
+                                                         float* __restrict__ part, int64_t C, int64_t len, float slope, int64_t row0) {
+  constexpr int N = Vec<T>::N;
+  __shared__ float red[4][2];
+  const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
+  const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+  float s1 = 0.f, s2 = 0.f;
+#pragma unroll 4
+  for (int64_t c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
+    float v[N], g[N], wv[N], bv[N];
+    load(x + row * C, c, hi, v);
+    load(gy + row * C, c, hi, g);
+    load_f<N>(w, c, hi, 1.f, wv);
+    load_f<N>(b, c, hi, 0.f, bv);
+    float t1 = 0.f, t2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float xh = (v[e] - mean) * rstd;
+      const float h = (fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope) * wv[e];
+      t1 += h;
+      t2 = c + e < hi ? fmaf(h, xh, t2) : t2;
+    }
+    s1 += t1;
+    s2 += t2;
+  }
+  s1 = lane_sum<64>(s1);
+  s2 = lane_sum<64>(s2);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6][0] = s1;
+    red[threadIdx.x >> 6][1] = s2;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2)
+    part[(row * gridDim.x + blockIdx.x) * 2 + threadIdx.x] =
+        (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// sums[row] = the row's means of h and h xhat
+__global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict__ part, int chunks, int64_t C, float* __restrict__ sums,
+                                                        int64_t row0) {
+  __shared__ float red[4][2];
+  const int64_t row = row0 + blockIdx.x;
+  float s1 = 0.f, s2 = 0.f;
+  for (int i = threadIdx.x; i < chunks; i += 256) {
+    s1 += part[(row * chunks + i) * 2];
+    s2 += part[(row * chunks + i) * 2 + 1];
+  }
+  s1 = lane_sum<64>(s1);
+  s2 = lane_sum<64>(s2);
+  if ((threadIdx.x & 63) == 0) {
+    red[threadIdx.x >> 6][0] = s1;
+    red[threadIdx.x >> 6][1] = s2;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2)
+    sums[row * 2 + threadIdx.x] =
+        ((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x])) / (float)C;
+}
+
+// columns of a workgroup, rows [blockIdx.y * span, + span): gx, and the columns' sums over these rows
+template <class T>
+__global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                        const T* __restrict__ gy, const float* __restrict__ stats,
+                                                        const float* __restrict__ sums, T* __restrict__ gx, float* __restrict__ gw,
+                                                        float* __restrict__ gb, int64_t stride, int64_t rows, int64_t span, int64_t C,
+                                                        float slope) {
+  constexpr int N = Vec<T>::N;
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
+  const int64_t lo = blockIdx.y * span, hi = min(rows, lo + span);
+  if (c >= C) return;
+  float wv[N], bv[N], aw[N], ab[N];
+  load_f<N>(w, c, C, 1.f, wv);
+  load_f<N>(b, c, C, 0.f, bv);
+#pragma unroll
+  for (int e = 0; e < N; ++e) aw[e] = ab[e] = 0.f;
+#pragma unroll 2
+  for (int64_t r = lo; r < hi; ++r) {
+    float v[N], g[N];
+    load(x + r * C, c, C, v);
+    load(gy + r * C, c, C, g);
+    const float mean = stats[2 * r], rstd = stats[2 * r + 1], s1 = sums[2 * r], s2 = sums[2 * r + 1];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float xh = (v[e] - mean) * rstd;
+      const float gg = fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope;
+      aw[e] = fmaf(gg, xh, aw[e]);
+      ab[e] += gg;
+      v[e] = rstd * (gg * wv[e] - fmaf(xh, s2, s1));
+    }
+    if (gx) store(gx + r * C, c, C, v);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (c + e < C) {
+      if (gw) gw[blockIdx.y * stride + c + e] = aw[e];
+      if (gb) gb[blockIdx.y * stride + c + e] = ab[e];
+    }
+}
+
+// ---------------------------------------------------------------- host
+constexpr int64_t kRowsPerLaunch = 32768;     // a grid's y extent is below 65536
+
+// columns of a chunk: about 1024 chunks in all, 4096 to 16384 columns each (a multiple of 4096), at most 1024 to a row
+int64_t chunk_len(int64_t rows, int64_t cols) {
+  int64_t len = 16384;
+  while (len > 4096 && rows * ((cols + len - 1) / len) < 1024) len >>= 1;
+  const int64_t least = ((cols + 1023) / 1024 + 4095) / 4096 * 4096;
+  return len > least ? len : least;
+}
+int64_t chunks_of(int64_t rows, int64_t cols) { return (cols + chunk_len(rows, cols) - 1) / chunk_len(rows, cols); }
+// row groups of the last pass: enough workgroups for the chip, at least 4 rows each
+int64_t groups_of(int64_t rows, int64_t cols) {
+  const int64_t wide = (cols + 1023) / 1024;
+  int64_t g = (1024 + wide - 1) / wide;
+  if (g > rows / 4) g = rows / 4;
+  return g < 1 ? 1 : g > 256 ? 256 : g;
+}
+
+// lanes of a row: the fewest that hold it with 16 bytes each, up to a wave; then up to 16 elements each; then workgroups
+struct Shape { int G, E, NT; };
+Shape shape_of(int64_t cols, int vec) {
+  for (int G = 4; G <= 64; G *= 2)
+    if (cols <= (int64_t)G * vec) return {G, vec, 256};
+  for (int E = 8; E <= 16; E *= 2)
+    if (E > vec && cols <= 64 * E) return {64, E, 256};
+  for (int G = 256; G <= 1024; G *= 4)
+    for (int E = 8; E <= 16; E *= 2)
+      if (cols <= (int64_t)G * E) return {G, E, G};
+  return {0, 0, 0};
+}
+int64_t resident_blocks(int64_t rows, const Shape& s) {
+  const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb;
+  const int64_t most = s.NT == 1024 ? kBlocks / 4 : kBlocks;
+  return need < most ? need : most;
+}
+
+bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && rows <= (int64_t)1 << 40 && cols <= (int64_t)1 << 31; }
+
+int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
+
+template <class T, int G, int K, int NT>
+void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, int64_t rows, int64_t cols, float eps, float slope,
+                hipStream_t st) {
+  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}));
+  const float inv = 1.0f / (float)cols;
+  if (cols % Vec<T>::N) hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, true>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
+  else hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, false>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
+}
+template <class T, int G, int K, int NT>
+void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* part, int64_t rows, int64_t cols, float eps,
+                float slope, hipStream_t st) {
+  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}));
+  const float inv = 1.0f / (float)cols;
+  if (cols % Vec<T>::N) hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, true>), grid, dim3(NT), 0, st, x, w, b, gy, gx, part, rows, (int)cols, inv, eps, slope);
+  else hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, false>), grid, dim3(NT), 0, st, x, w, b, gy, gx, part, rows, (int)cols, inv, eps, slope);
+}
+
+#define LR_LN_SHAPES(CALL)                                                                          \
+  const Shape s = shape_of(cols, Vec<T>::N);                                                        \
+  constexpr int N = Vec<T>::N;                                                                      \
+  if (s.G == 4) CALL(4, 1, 256);                                                                    \
+  else if (s.G == 8) CALL(8, 1, 256);                                                               \
+  else if (s.G == 16) CALL(16, 1, 256);                                                             \
+  else if (s.G == 32) CALL(32, 1, 256);                                                             \
+  else if (s.G == 64 && s.E == N) CALL(64, 1, 256);                                                 \
+  else if (s.G == 64 && s.E == 8) CALL(64, 8 / N, 256);                                             \
+  else if (s.G == 64) CALL(64, 16 / N, 256);                                                        \
+  else if (s.G == 256 && s.E == 8) CALL(256, 8 / N, 256);                                           \
+  else if (s.G == 256) CALL(256, 16 / N, 256);                                                      \
+  else if (s.E == 8) CALL(1024, 8 / N, 1024);                                                       \
+  else CALL(1024, 16 / N, 1024)
+
+template <class T>
+int fwd(const T* x, const float* w, const float* b, T* y, float* stats, float* ws, int64_t rows, int64_t cols, float eps, float slope,
+        hipStream_t st) {
+  if (cols <= kResident) {
+#define LR_CALL(G, K, NT) launch_fwd<T, G, K, NT>(x, w, b, y, stats, rows, cols, eps, slope, st)
+    LR_LN_SHAPES(LR_CALL);
+#undef LR_CALL
+    return lr_launch_status();
+  }
+  const int64_t len = chunk_len(rows, cols), chunks = chunks_of(rows, cols);
+  float* sv = stats ? stats : ws + 2 * rows * chunks;
+  for (int64_t r = 0; r < rows; r += kRowsPerLaunch) {
+    const unsigned k = (unsigned)(rows - r < kRowsPerLaunch ? rows - r : kRowsPerLaunch);
+    hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
+    hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, len, eps, sv, r);
+    hipLaunchKernelGGL((chunk_fwd_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, y, sv, cols, len, slope, r);
+    const int rc = lr_launch_status();
+    if (rc != LR_OK) return rc;
+  }
+  return LR_OK;
+}
+
+template <class T>
+int bwd(const T* x, const float* w, const float* b, const T* gy, const float* stats, T* gx, float* gw, float* gb, float* ws,
+        int64_t rows, int64_t cols, float eps, float slope, hipStream_t st) {
+  const unsigned fin = (unsigned)((2 * cols + kFinish - 1) / kFinish);
+  if (cols <= kResident) {
+    float* part = gw || gb ? ws : nullptr;
+#define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, part, rows, cols, eps, slope, st)
+    LR_LN_SHAPES(LR_CALL);
+#undef LR_CALL
+    const int rc = lr_launch_status();
+    if (rc != LR_OK || !part) return rc;
+    hipLaunchKernelGGL(finish_kernel, dim3(fin), dim3(1024), 0, st, part, (int)resident_blocks(rows, s), cols, gw, gb);
+    return lr_launch_status();
+  }
+  const int64_t len = chunk_len(rows, cols), chunks = chunks_of(rows, cols), groups = groups_of(rows, cols);
+  float* sums = ws + 2 * rows * chunks;
+  float* own = sums + up16(2 * rows);
+  float* part = own + up16(2 * rows);
+  for (int64_t r = 0; r < rows; r += kRowsPerLaunch) {
+    const unsigned k = (unsigned)(rows - r < kRowsPerLaunch ? rows - r : kRowsPerLaunch);
+    if (!stats) {
+      hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
+      hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, len, eps, own, r);
+    }
+    hipLaunchKernelGGL((chunk_sums_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, stats ? stats : own, ws, cols, len, slope, r);
+    hipLaunchKernelGGL(join_sums_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, sums, r);
+    const int rc = lr_launch_status();
+    if (rc != LR_OK) return rc;
+  }
+  const int64_t span = (rows + groups - 1) / groups;
+  const int64_t wide = (cols + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N);
+  const bool direct = groups == 1;
+  hipLaunchKernelGGL((chunk_bwd_kernel<T>), dim3((unsigned)wide, (unsigned)groups), dim3(256), 0, st, x, w, b, gy, stats ? stats : own, sums, gx,
+                     direct ? gw : part, direct ? gb : part + cols, direct ? 0 : 2 * cols, rows, span, cols, slope);
+  int rc = lr_launch_status();
+  if (rc != LR_OK || direct || !(gw || gb)) return rc;
+  hipLaunchKernelGGL(finish_kernel, dim3(fin), dim3(1024), 0, st, part, (int)groups, cols, gw, gb);
+  return lr_launch_status();
+}
+
+__global__ __launch_bounds__(256) void zero_kernel(float* a, float* b, int64_t n) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    if (a) a[i] = 0.f;
+    if (b) b[i] = 0.f;
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t lr_layer_norm_resident_cols(void) { return kResident; }
+
+extern "C" int64_t lr_layer_norm_workspace(int64_t rows, int64_t cols, int backward) {
+  if (!sizes_ok(rows, cols)) return LR_EINVAL;
+  if (rows == 0) return 0;
+  if (cols <= kResident) {
+    if (!backward) return 0;
+    // the larger of the two types' launches
+    const int64_t a = resident_blocks(rows, shape_of(cols, 4)), b = resident_blocks(rows, shape_of(cols, 8));
+    return 4 * 2 * cols * (a > b ? a : b);
+  }
+  const int64_t words = 2 * rows * chunks_of(rows, cols);
+  if (!backward) return 4 * (words + 2 * rows);
+  const int64_t groups = groups_of(rows, cols);
+  return 4 * (words + 2 * up16(2 * rows) + (groups > 1 ? 2 * cols * groups : 0));
+}
+
+extern "C" int lr_layer_norm(const void* x, const float* w, const float* b, void* y, float* stats, void* workspace, int64_t rows,
+                             int64_t cols, int bf16, float eps, float slope, void* stream) {
+  if (!sizes_ok(rows, cols) || !(eps >= 0.f)) return LR_EINVAL;
+  if (rows == 0) return LR_OK;
+  if (!x || !y || (cols > kResident && !workspace)) return LR_ENULL;
+  hipStream_t st = lr_stream(stream);
+  float* ws = static_cast<float*>(workspace);
+  if (bf16) return fwd(static_cast<const uint16_t*>(x), w, b, static_cast<uint16_t*>(y), stats, ws, rows, cols, eps, slope, st);
+  return fwd(static_cast<const float*>(x), w, b, static_cast<float*>(y), stats, ws, rows, cols, eps, slope, st);
+}
+
+extern "C" int lr_layer_norm_bwd(const void* x, const float* w, const float* b, const void* gy, const float* stats, void* gx, float* gw,
+                                 float* gb, void* workspace, int64_t rows, int64_t cols, int bf16, float eps, float slope, void* stream) {
+  if (!sizes_ok(rows, cols) || !(eps >= 0.f)) return LR_EINVAL;
+  hipStream_t st = lr_stream(stream);
+  if (rows == 0) {
+    if (!gw && !gb) return LR_OK;
+    hipLaunchKernelGGL(zero_kernel, dim3((unsigned)((cols + 255) / 256 < 1024 ? (cols + 255) / 256 : 1024)), dim3(256), 0, st, gw, gb, cols);
+    return lr_launch_status();
+  }
+  if (!gx && !gw && !gb) return LR_OK;
+  if (!x || !gy || !workspace) return LR_ENULL;
+  float* ws = static_cast<float*>(workspace);
+  if (bf16)
+    return bwd(static_cast<const uint16_t*>(x), w, b, static_cast<const uint16_t*>(gy), stats, static_cast<uint16_t*>(gx), gw, gb, ws, rows,
+               cols, eps, slope, st);
+  return bwd(static_cast<const float*>(x), w, b, static_cast<const float*>(gy), stats, static_cast<float*>(gx), gw, gb, ws, rows, cols, eps,
+             slope, st);
+}

@@ -1,0 +1,524 @@
+// optim.hip — the update of the network's parameters: the AdamW step over all the tensors of a model in one launch (64 tensors a
+// launch), with 32-bit or block-scaled 8-bit states, and the global norm of the gradients it clips by.
+//
+// The reference trains with torch.optim.Adam (src/liftreg/networks/RegistrationNet.py:245); with weight_decay = 0 this is its step.
+//   g = grad * c,  c = min(1, max_norm / (|grad|_2 + 1e-6))         (c = 1 without clipping)
+//   m = b1 m + (1 - b1) g,   v = b2 v + (1 - b2) g^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit states: 32 consecutive elements of a tensor share a power-of-two scale 2^(s - 127) (one byte, e8m0); m / scale is held in
+// e4m3, v / scale in e5m2.  Both are rounded stochastically: a step moves v by (1 - b2) = 0.1 % of itself while neighbouring codes
+// are 12 ... 25 % apart, so rounding to nearest would leave v where it is for ever; rounding up with the probability of the
+// remainder keeps the expected state equal to the unrounded one.  A v that is not zero never rounds to zero (m / eps would follow).
+// The block's largest magnitude is placed in [2^7, 2^8) of e4m3's 448 and in [2^14, 2^15) of e5m2's 57344: rounding up cannot
+// overflow.  The 16 + 16 random bits of an element are a hash of (seed, step, position), so a step can be repeated bit for bit.
+// m and v are formed with the separate roundings of the formula above (no contraction), so that the states do not depend on the
+// compiler; the update itself uses v_sqrt_f32 / v_rcp_f32 (1 ulp each, of a number that is lr times smaller than p).
+#include "lr_common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPerThread = 16;                      // elements of a chunk per thread: 4 vectors of 4
+constexpr int kChunk = kThreads * kPerThread;       // a whole number of 32-element scale blocks
+constexpr int kTensors = 64;                        // tensors of one launch: a lane each in the search for a chunk's tensor
+constexpr int kNormBlocks = 512;
+
+// tensors of one launch, by value in the kernel arguments (at most 4 KB): nothing to upload, nothing that a captured graph could
+// outlive
+struct Table32 {
+  static constexpr int kMax = kTensors;
+  void* p[kMax];
+  const void* g[kMax];
+  float* m[kMax];
+  float* v[kMax];
+  int64_t n[kMax];
+  uint32_t end[kMax];   // chunks of this launch up to and including this tensor
+  int count;
+};
+struct Table8 {
+  static constexpr int kMax = 56;
+  void* p[kMax];
+  const void* g[kMax];
+  uint8_t* m[kMax];
+  uint8_t* v[kMax];
+  uint8_t* ms[kMax];
+  uint8_t* vs[kMax];
+  int64_t n[kMax];
+  uint32_t end[kMax];
+  uint32_t pos[kMax];   // position of the tensor's first element in the concatenation padded to whole scale blocks, mod 2^32
+  int count;
+};
+struct TableG {
+  static constexpr int kMax = kTensors;
+  const void* g[kMax];
+  int64_t n[kMax];
+  uint32_t end[kMax];
+  int count;
+};
+static_assert(sizeof(Table32) <= 3840 && sizeof(Table8) <= 3968 && sizeof(TableG) <= 3840, "kernel arguments are 4 KB");
+
+struct Rates {               // what a step derives from its hyperparameters
+  float size, rbc2, keep;
+  uint32_t key;
+};
+struct Hyper {
+  double b1, b2, lr, eps, wd;
+  Rates r;                   // of (lr, step); derived on the device where one of them lives there
+  const float* lr_dev;       // if set: the learning rate
+  const int64_t* step_dev;   // if set: the step
+  int64_t step;
+  const double* sumsq;       // partial sums of squares of the gradients (n_sumsq of them), or NULL
+  const float* norm_in;      // the gradients' norm, or NULL
+  float* norm_out;
+  int n_sumsq;
+  float max_norm;
+  uint64_t seed;
+};
+
+// the alignment of a tensor that is a view into a flat buffer is its element's: gfx950 loads 16 bytes from any dword (or byte)
+// address in one instruction, aligned or not at the same rate where the access is contiguous over the wave
+typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t h4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u1 __attribute__((aligned(1)));
+
+struct F32 { float x[4]; };
+
+__device__ __forceinline__ float bf_to_f(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
+__device__ __forceinline__ uint16_t f_to_bf(float f) {   // nearest even; NaN stays NaN
+  const uint32_t u = __float_as_uint(f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+
+// 4 elements at i of an array of n (elements past the end read as 0 and are not written)
+__device__ __forceinline__ F32 load4(const float* a, int64_t i, int64_t n) {
+  F32 r = {{0.f, 0.f, 0.f, 0.f}};
+  if (i + 4 <= n) {
+    const f4 t = *reinterpret_cast<const f4*>(a + i);
+    r.x[0] = t[0]; r.x[1] = t[1]; r.x[2] = t[2]; r.x[3] = t[3];
+  } else {
+    for (int k = 0; k < 3; ++k)
+      if (i + k < n) r.x[k] = a[i + k];
+  }
+  return r;
+}
+__device__ __forceinline__ F32 load4(const uint16_t* a, int64_t i, int64_t n) {
+  F32 r = {{0.f, 0.f, 0.f, 0.f}};
+  if (i + 4 <= n) {
+    const h4 t = *reinterpret_cast<const h4*>(a + i);
+    for (int k = 0; k < 4; ++k) r.x[k] = bf_to_f(t[k]);
+  } else {
+    for (int k = 0; k < 3; ++k)
+      if (i + k < n) r.x[k] = bf_to_f(a[i + k]);
+  }
+  return r;
+}
+__device__ __forceinline__ void store4(float* a, int64_t i, int64_t n, const F32& r) {
+  if (i + 4 <= n) {
+    f4 t = {r.x[0], r.x[1], r.x[2], r.x[3]};
+    *reinterpret_cast<f4*>(a + i) = t;
+  } else {
+    for (int k = 0; k < 3; ++k)
+      if (i + k < n) a[i + k] = r.x[k];
+  }
+}
+__device__ __forceinline__ void store4(uint16_t* a, int64_t i, int64_t n, const F32& r) {
+  if (i + 4 <= n) {
+    h4 t = {f_to_bf(r.x[0]), f_to_bf(r.x[1]), f_to_bf(r.x[2]), f_to_bf(r.x[3])};
+    *reinterpret_cast<h4*>(a + i) = t;
+  } else {
+    for (int k = 0; k < 3; ++k)
+      if (i + k < n) a[i + k] = f_to_bf(r.x[k]);
+  }
+}
+__device__ __forceinline__ uint32_t load4b(const uint8_t* a, int64_t i, int64_t n) {
+  if (i + 4 <= n) return *reinterpret_cast<const u1*>(a + i);
+  uint32_t r = 0;
+  for (int k = 0; k < 3; ++k)
+    if (i + k < n) r |= (uint32_t)a[i + k] << (8 * k);
+  return r;
+}
+__device__ __forceinline__ void store4b(uint8_t* a, int64_t i, int64_t n, uint32_t r) {
+  if (i + 4 <= n) *reinterpret_cast<u1*>(a + i) = r;
+  else
+    for (int k = 0; k < 3; ++k)
+      if (i + k < n) a[i + k] = (uint8_t)(r >> (8 * k));
+}
+
+// the tensor that chunk c belongs to: lane k holds the end of tensor k
+__device__ __forceinline__ int tensor_of(uint32_t end_of_lane, uint32_t c) {
+  return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(end_of_lane <= c)));
+}
+template <class T>
+__device__ __forceinline__ uint32_t lane_end(const T& t) {
+  const int lane = threadIdx.x & 63;
+  return lane < t.count ? t.end[min(lane, T::kMax - 1)] : 0xffffffffu;
+}
+
+__device__ __forceinline__ double block_sum(double s) {   // the same order in every block: the same bits
+  __shared__ double red[kThreads / 64];
+  s = lr_wave_sum(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ---------------------------------------------------------------- the gradients' norm
+// fp64 accumulators: 13 M squares of numbers that span decades; the conversion and the fma hide under the read.
+template <class G>
+__global__ __launch_bounds__(kThreads) void sumsq_kernel(TableG t, double* __restrict__ partial) {
+  const uint32_t ends = lane_end(t), chunks = t.end[t.count - 1];
+  double s = 0.0;
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int k = tensor_of(ends, c);
+    const int64_t n = t.n[k], base = (int64_t)(c - (k ? t.end[k - 1] : 0u)) * kChunk;
+    const G* g = static_cast<const G*>(t.g[k]);
+    F32 x[kPerThread / 4];
+#pragma unroll
+    for (int j = 0; j < kPerThread / 4; ++j) x[j] = load4(g, base + (j * kThreads + threadIdx.x) * 4, n);
+#pragma unroll
+    for (int j = 0; j < kPerThread / 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s = fma((double)x[j].x[e], (double)x[j].x[e], s);
+  }
+  s = block_sum(s);
+  if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(kThreads) void norm_kernel(const double* __restrict__ partial, int n, float* __restrict__ out) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += kThreads) s += partial[i];
+  s = block_sum(s);
+  if (threadIdx.x == 0) *out = (float)sqrt(s);
+}
+
+// ---------------------------------------------------------------- 8-bit states
+__host__ __device__ inline uint32_t mix(uint32_t x) {   // xor-shift and odd multiplication, twice: a bijection of 32 bits
+  x ^= x >> 16;
+  x *= 0x0A00F875u;
+  x ^= x >> 15;
+  x *= 0x517B5965u;
+  return x ^ (x >> 16);
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true));
+}
+// over the 8 lanes that hold a scale block: neighbours, pairs, then the mirrored half row
+__device__ __forceinline__ uint32_t max8(uint32_t x) { return max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(x))); }
+
+__device__ __forceinline__ float scale_of(uint32_t s) {   // 2^(s - 127); 255 is NaN, 0 the subnormal 2^-127
+  const uint32_t b = s == 255u ? 0x7fc00000u : s == 0u ? 0x00400000u : s << 23;
+  return __uint_as_float(b);
+}
+
+// the exponent byte of the block's scale: its peak lands in [2^top, 2^(top+1))
+template <int TOP>
+__device__ __forceinline__ uint32_t block_scale(const F32& a) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) u = max(u, __float_as_uint(a.x[e]) & 0x7fffffffu);
+  const int ex = (int)(max8(u) >> 23);
+  return ex == 255 ? 255u : (uint32_t)max(ex - TOP, 1);
+}
+
+// |x| / scale in MAN mantissa bits, exponent bias BIAS, rounded up with the probability of what is cut off
+template <int MAN, int BIAS>
+__device__ __forceinline__ uint32_t code_of(float x, float inv, uint32_t r) {
+  const float y = fabsf(x) * inv;
+  const uint32_t normal = ((__float_as_uint(y) + (r << (23 - MAN - 16))) >> (23 - MAN)) - ((127u - BIAS) << MAN);
+  const uint32_t low = (uint32_t)(y * (float)(1u << (BIAS - 1 + MAN)) + (float)r * 0x1p-16f);
+  return y >= __uint_as_float((128u - BIAS) << 23) ? normal : low;
+}
+
+typedef float f2 __attribute__((ext_vector_type(2)));
+
+template <class T>
+struct State;   // how a step reads and writes the two moments of 4 elements
+
+template <>
+struct State<Table32> {
+  F32 m, v;
+  __device__ __forceinline__ void load(const Table32& t, int k, int64_t i, int64_t n) {
+    m = load4(t.m[k], i, n);
+    v = load4(t.v[k], i, n);
+  }
+  __device__ __forceinline__ void open() {}
+  __device__ __forceinline__ void store(const Table32& t, int k, int64_t i, int64_t n, uint32_t) {
+    store4(t.m[k], i, n, m);
+    store4(t.v[k], i, n, v);
+  }
+};
+
+template <>
+struct State<Table8> {
+  F32 m, v;
+  uint32_t mq, vq, ms, vs;
+  __device__ __forceinline__ void load(const Table8& t, int k, int64_t i, int64_t n) {
+    mq = load4b(t.m[k], i, n);
+    vq = load4b(t.v[k], i, n);
+    ms = i < n ? t.ms[k][i >> 5] : 1u;
+    vs = i < n ? t.vs[k][i >> 5] : 1u;
+  }
+  __device__ __forceinline__ void open() {
+    const float a = scale_of(ms), b = scale_of(vs);
+    const f2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq, true);
+    const f2 v0 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vq, false), v1 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vq, true);
+    m.x[0] = m0[0] * a; m.x[1] = m0[1] * a; m.x[2] = m1[0] * a; m.x[3] = m1[1] * a;
+    v.x[0] = v0[0] * b; v.x[1] = v0[1] * b; v.x[2] = v1[0] * b; v.x[3] = v1[1] * b;
+  }
+  // every lane of the wave comes here (elements past the end are zeros): the scale is a maximum over 8 lanes
+  __device__ __forceinline__ void store(const Table8& t, int k, int64_t i, int64_t n, uint32_t key) {
+    ms = block_scale<7>(m);
+    vs = block_scale<14>(v);
+    const float a = ms == 255u ? 0.f : __uint_as_float((254u - ms) << 23), b = vs == 255u ? 0.f : __uint_as_float((254u - vs) << 23);
+    uint32_t cm = 0, cv = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t r = mix((t.pos[k] + (uint32_t)i + e) ^ key);
+      const float x = ms == 255u ? 0.f : m.x[e], w = vs == 255u ? 0.f : v.x[e];   // a block that is not finite: scale NaN, codes 0
+      cm |= (code_of<3, 7>(x, a, r & 0xffffu) | ((__float_as_uint(x) >> 24) & 0x80u)) << (8 * e);
+      const uint32_t c = code_of<2, 15>(w, b, r >> 16);
+      cv |= (w > 0.f ? max(c, 1u) : c) << (8 * e);
+    }
+    store4b(t.m[k], i, n, cm);
+    store4b(t.v[k], i, n, cv);
+    if ((threadIdx.x & 7) == 0 && i < n) {
+      t.ms[k][i >> 5] = (uint8_t)ms;
+      t.vs[k][i >> 5] = (uint8_t)vs;
+    }
+  }
+};
+
+__host__ __device__ inline double ipow(double b, int64_t t) {   // b^t, t >= 0
+  double r = 1.0;
+  for (; t > 0; t >>= 1) {
+    if (t & 1) r *= b;
+    b *= b;
+  }
+  return r;
+}
+__host__ __device__ inline Rates rates(const Hyper& h, double lr, int64_t step) {
+  Rates r;
+  r.size = (float)(lr / (1.0 - ipow(h.b1, step)));
+  r.rbc2 = (float)(1.0 / sqrt(1.0 - ipow(h.b2, step)));
+  r.keep = (float)(1.0 - lr * h.wd);
+  r.key = mix(mix(mix((uint32_t)step) ^ (uint32_t)(h.seed >> 32)) ^ (uint32_t)h.seed);
+  return r;
+}
+
+// Bound by memory: 28 bytes an element with 32-bit states and fp32 parameters, 16 with 8-bit ones.
+template <class P, class T>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
+  const uint32_t ends = lane_end(t), chunks = t.end[t.count - 1];
+  Rates r = h.r;
+  if (h.lr_dev || h.step_dev) r = rates(h, h.lr_dev ? (double)*h.lr_dev : h.lr, h.step_dev ? *h.step_dev : h.step);
+  const float b1 = (float)h.b1, b2 = (float)h.b2, c1 = (float)(1.0 - h.b1), c2 = (float)(1.0 - h.b2);
+  const float eps = (float)h.eps;
+  float coef = 1.0f;
+  if (h.sumsq || h.norm_in) {
+    float norm;
+    if (h.sumsq) {
+      double s = 0.0;
+      for (int i = threadIdx.x; i < h.n_sumsq; i += kThreads) s += h.sumsq[i];
+      norm = (float)sqrt(block_sum(s));
+      if (blockIdx.x == 0 && threadIdx.x == 0 && h.norm_out) *h.norm_out = norm;
+    } else {
+      norm = *h.norm_in;
+    }
+    coef = h.max_norm / (norm + 1e-6f);
+    coef = coef > 1.0f ? 1.0f : coef;     // NaN stays NaN
+  }
+  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const int k = tensor_of(ends, c);
+    const int64_t n = t.n[k], base = (int64_t)(c - (k ? t.end[k - 1] : 0u)) * kChunk;
+    P* pp = static_cast<P*>(t.p[k]);
+    const P* gp = static_cast<const P*>(t.g[k]);
+#pragma unroll
+    for (int j = 0; j < kPerThread / 4; j += 2) {
+      F32 p[2], g[2];
+      State<T> s[2];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
+        g[q] = load4(gp, i, n);
+        s[q].load(t, k, i, n);
+        p[q] = load4(pp, i, n);
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
+        s[q].open();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = g[q].x[e] * coef;
+          const float m = s[q].m.x[e] * b1 + x * c1, v = s[q].v.x[e] * b2 + x * x * c2;
+          s[q].m.x[e] = m;
+          s[q].v.x[e] = v;
+          const float den = fmaf(__builtin_amdgcn_sqrtf(v), r.rbc2, eps);
+          p[q].x[e] = p[q].x[e] * r.keep - r.size * (m * __builtin_amdgcn_rcpf(den));
+        }
+        store4(pp, i, n, p[q]);
+        s[q].store(t, k, i, n, r.key);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+uint32_t chunks_of(int64_t n) { return (uint32_t)((n + kChunk - 1) / kChunk); }
+
+bool sizes_ok(const int64_t* numel, int n) {
+  if (n < 1) return false;
+  for (int i = 0; i < n; ++i)
+    if (numel[i] < 0 || numel[i] > (int64_t)1 << 40) return false;
+  return true;
+}
+
+// calls f(first, last, chunks) for each run of at most `most` tensors with elements
+template <class F>
+int for_launches(const int64_t* numel, int n, int most, F f) {
+  int first = 0;
+  while (first < n) {
+    int last = first, held = 0;
+    int64_t chunks = 0;
+    while (last < n && held < most) {
+      const int64_t more = chunks_of(numel[last]);
+      if (chunks + more > 0x7fffffff) break;
+      chunks += more;
+      held += numel[last] > 0;
+      ++last;
+    }
+    if (held) {
+      const int rc = f(first, last, (uint32_t)chunks);
+      if (rc != LR_OK) return rc;
+    }
+    first = last;
+  }
+  return LR_OK;
+}
+
+unsigned norm_blocks(uint32_t chunks) { return chunks < (uint32_t)kNormBlocks ? chunks : (unsigned)kNormBlocks; }
+
+int sumsq_launches(const void* const* grads, const int64_t* numel, int n, int bf16, double* partial, hipStream_t st) {
+  int used = 0;
+  return for_launches(numel, n, TableG::kMax, [&](int first, int last, uint32_t chunks) {
+    TableG t;
+    int k = 0;
+    uint32_t end = 0;
+    for (int i = first; i < last; ++i) {
+      if (!numel[i]) continue;
+      t.g[k] = grads[i];
+      t.n[k] = numel[i];
+      t.end[k++] = end += chunks_of(numel[i]);
+    }
+    t.count = k;
+    const unsigned nb = norm_blocks(chunks);
+    if (bf16) hipLaunchKernelGGL((sumsq_kernel<uint16_t>), dim3(nb), dim3(kThreads), 0, st, t, partial + used);
+    else hipLaunchKernelGGL((sumsq_kernel<float>), dim3(nb), dim3(kThreads), 0, st, t, partial + used);
+    used += (int)nb;
+    return lr_launch_status();
+  });
+}
+
+}  // namespace
+
+extern "C" int64_t lr_grad_norm_partials(const int64_t* numel, int n) {
+  if (!numel) return LR_ENULL;
+  if (!sizes_ok(numel, n)) return LR_EINVAL;
+  int64_t used = 0;
+  for_launches(numel, n, TableG::kMax, [&](int, int, uint32_t chunks) {
+    used += norm_blocks(chunks);
+    return LR_OK;
+  });
+  return used;
+}
+
+extern "C" int lr_grad_norm(const void* const* grads, const int64_t* numel, int n, int bf16, double* partial, float* norm,
+                            void* stream) {
+  if (!grads || !numel || !partial || !norm) return LR_ENULL;
+  const int64_t used = lr_grad_norm_partials(numel, n);
+  if (used < 0) return (int)used;
+  for (int i = 0; i < n; ++i)
+    if (numel[i] && !grads[i]) return LR_ENULL;
+  hipStream_t st = lr_stream(stream);
+  const int rc = sumsq_launches(grads, numel, n, bf16, partial, st);
+  if (rc != LR_OK) return rc;
+  hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, partial, (int)used, norm);
+  return lr_launch_status();
+}
+
+extern "C" int lr_adamw_step(void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq,
+                             void* const* exp_avg_scale, void* const* exp_avg_sq_scale, const int64_t* numel, int n, int bf16,
+                             double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step,
+                             const float* lr_dev, const int64_t* step_dev, float max_norm, const float* norm_in,
+                             double* partial, float* norm_out, uint64_t seed, void* stream) {
+  if (!params || !grads || !exp_avg || !exp_avg_sq || !numel) return LR_ENULL;
+  if (!exp_avg_scale != !exp_avg_sq_scale) return LR_ENULL;
+  if (!sizes_ok(numel, n)) return LR_EINVAL;
+  if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0) || (!step_dev && step < 1)) return LR_EINVAL;
+  if ((norm_in || partial) && !(max_norm > 0)) return LR_EINVAL;
+  if (norm_in && partial) return LR_EINVAL;
+  const bool eight = exp_avg_scale != nullptr;
+  for (int i = 0; i < n; ++i)
+    if (numel[i] && (!params[i] || !grads[i] || !exp_avg[i] || !exp_avg_sq[i] || (eight && (!exp_avg_scale[i] || !exp_avg_sq_scale[i]))))
+      return LR_ENULL;
+  hipStream_t st = lr_stream(stream);
+  Hyper h = {beta1, beta2, lr, eps, weight_decay, {}, lr_dev, step_dev, step, partial, norm_in, norm_out, 0, max_norm, seed};
+  h.r = rates(h, lr, step_dev ? 1 : step);
+  if (partial) {
+    h.n_sumsq = (int)lr_grad_norm_partials(numel, n);
+    const int rc = sumsq_launches(grads, numel, n, bf16, partial, st);
+    if (rc != LR_OK) return rc;
+    if (!h.n_sumsq && norm_out) {     // no element at all: the norm is 0
+      hipLaunchKernelGGL(norm_kernel, dim3(1), dim3(kThreads), 0, st, partial, 0, norm_out);
+      return lr_launch_status();
+    }
+  }
+  // 2048 blocks of four waves: every wave slot of the 256 CUs
+  auto grid = [](uint32_t chunks) { return dim3(chunks < 2048u ? chunks : 2048u); };
+  if (!eight)
+    return for_launches(numel, n, Table32::kMax, [&](int first, int last, uint32_t chunks) {
+      Table32 t;
+      int k = 0;
+      uint32_t end = 0;
+      for (int i = first; i < last; ++i) {
+        if (!numel[i]) continue;
+        t.p[k] = params[i];
+        t.g[k] = grads[i];
+        t.m[k] = static_cast<float*>(exp_avg[i]);
+        t.v[k] = static_cast<float*>(exp_avg_sq[i]);
+        t.n[k] = numel[i];
+        t.end[k++] = end += chunks_of(numel[i]);
+      }
+      t.count = k;
+      if (bf16) hipLaunchKernelGGL((adamw_kernel<uint16_t, Table32>), grid(chunks), dim3(kThreads), 0, st, t, h);
+      else hipLaunchKernelGGL((adamw_kernel<float, Table32>), grid(chunks), dim3(kThreads), 0, st, t, h);
+      return lr_launch_status();
+    });
+  uint32_t pos = 0;
+  return for_launches(numel, n, Table8::kMax, [&](int first, int last, uint32_t chunks) {
+    Table8 t;
+    int k = 0;
+    uint32_t end = 0;
+    for (int i = first; i < last; ++i) {
+      if (!numel[i]) continue;
+      t.p[k] = params[i];
+      t.g[k] = grads[i];
+      t.m[k] = static_cast<uint8_t*>(exp_avg[i]);
+      t.v[k] = static_cast<uint8_t*>(exp_avg_sq[i]);
+      t.ms[k] = static_cast<uint8_t*>(exp_avg_scale[i]);
+      t.vs[k] = static_cast<uint8_t*>(exp_avg_sq_scale[i]);
+      t.n[k] = numel[i];
+      t.pos[k] = pos;
+      pos += (uint32_t)((numel[i] + 31) & ~(int64_t)31);
+      t.end[k++] = end += chunks_of(numel[i]);
+    }
+    t.count = k;
+    if (bf16) hipLaunchKernelGGL((adamw_kernel<uint16_t, Table8>), grid(chunks), dim3(kThreads), 0, st, t, h);
+    else hipLaunchKernelGGL((adamw_kernel<float, Table8>), grid(chunks), dim3(kThreads), 0, st, t, h);
+    return lr_launch_status();
+  });
+}

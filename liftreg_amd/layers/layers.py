@@ -9,8 +9,31 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from ..autograd import ConvBlockFn, LinearFn, NCCFn
+from ..autograd import ConvBlockFn, LayerNormFn, LinearFn, NCCFn
 from .._hip import NCC_SQUARED
+
+
+class LayerNorm(nn.Module):
+    """Layer norm over the trailing `normalized_shape` axes, with torch.nn.LayerNorm's arguments and state-dict keys, followed in
+    the same pass by LeakyReLU(negative_slope) (1.0: none).  Input float32 or bfloat16, weight and bias float32."""
+
+    def __init__(self, normalized_shape, eps=1e-5, elementwise_affine=True, bias=True, negative_slope=1.0):
+        super().__init__()
+        self.normalized_shape = (normalized_shape,) if isinstance(normalized_shape, numbers.Integral) else tuple(normalized_shape)
+        if not self.normalized_shape or min(self.normalized_shape) < 1:
+            raise ValueError(f"normalized_shape must name at least one axis of at least one element, got {normalized_shape}")
+        self.eps, self.negative_slope = float(eps), float(negative_slope)
+        self.weight = nn.Parameter(torch.ones(self.normalized_shape)) if elementwise_affine else None
+        self.bias = nn.Parameter(torch.zeros(self.normalized_shape)) if elementwise_affine and bias else None
+        self.premasked_grad = False      # set by the model where the consumer applies the LeakyReLU's mask (autograd.LayerNormFn)
+
+    def forward(self, x):
+        n = len(self.normalized_shape)
+        if tuple(x.shape[-n:]) != self.normalized_shape:
+            raise ValueError(f"the input's trailing axes must be {self.normalized_shape}, got shape {tuple(x.shape)}")
+        w, b = (None if t is None else t.reshape(-1) for t in (self.weight, self.bias))
+        y = LayerNormFn.apply(x.reshape(x.shape[:-n] + (-1,)) if n > 1 else x, w, b, self.eps, self.negative_slope, self.premasked_grad)
+        return y.view(x.shape) if n > 1 else y
 
 
 class convBlock(nn.Module):
@@ -18,11 +41,14 @@ class convBlock(nn.Module):
 
     `in_layout`/`out_layout` select NCDHW (the reference's layout, default) or channels-last
     NDHWC for activations that stay inside the encoder.
+
+    `layernorm`: Conv3d + layer norm over each voxel's channels + LeakyReLU, the last two in one pass (the reference's
+    block offers a batch norm there, which a batch of 1-8 volumes cannot feed).
     """
 
     def __init__(self, in_channels, out_channels, kernel_size=3, stride=1, padding=1, bias=True,
                  batchnorm=False, residual=False, nonlinear=nn.LeakyReLU(0.2),
-                 in_layout=ops.LAYOUT_NCDHW, out_layout=ops.LAYOUT_NCDHW):
+                 in_layout=ops.LAYOUT_NCDHW, out_layout=ops.LAYOUT_NCDHW, layernorm=False):
         super().__init__()
         if kernel_size != 3 or padding != 1 or batchnorm or residual:
             raise NotImplementedError("only the configuration the model uses is built: k3, p1, no BN/residual")
@@ -41,8 +67,20 @@ class convBlock(nn.Module):
             self._slope = float(nonlinear.negative_slope)
         else:
             raise NotImplementedError("fused epilogue supports LeakyReLU or None")
+        self.norm = None
+        if layernorm:
+            if out_layout not in (ops.LAYOUT_NCDHW, ops.LAYOUT_NDHWC):
+                raise ValueError("layernorm: out_layout must be LAYOUT_NCDHW or LAYOUT_NDHWC (a voxel's channels in one row)")
+            self.norm = LayerNorm(out_channels, negative_slope=self._slope)
 
     def forward(self, x, packed=None):
+        if self.norm is not None:
+            # the conv runs without activation and channels-last; its gradient is the one the norm hands back
+            y = ConvBlockFn.apply(x, self.conv.weight, self.conv.bias, self.stride, self.in_layout, ops.LAYOUT_NDHWC, 1.0, packed, True,
+                                  self.mask_input_slope)
+            self.norm.premasked_grad = self.premasked_grad
+            y = self.norm(y)
+            return y.permute(0, 4, 1, 2, 3).contiguous() if self.out_layout == ops.LAYOUT_NCDHW else y
         # Training, chained blocks: a 16-channel block whose consumer applies this block's LeakyReLU mask in its data
         # gradient (premasked_grad) also writes that mask as one byte per channel quad; it travels to the consumer as an
         # attribute of the activation tensor (`_lr_sign4`) and replaces the consumer's re-read of the activation.
@@ -60,9 +98,9 @@ class convBlock(nn.Module):
 
 
 class FullyConnectBlock(nn.Module):
-    """Linear + LeakyReLU(0.2) (layers/layers.py:413-439)."""
+    """Linear + LeakyReLU(0.2) (layers/layers.py:413-439); `layernorm`: Linear + layer norm over the features + LeakyReLU."""
 
-    def __init__(self, in_channels, out_channels, bias=True, nonlinear=nn.LeakyReLU(0.2)):
+    def __init__(self, in_channels, out_channels, bias=True, nonlinear=nn.LeakyReLU(0.2), layernorm=False):
         super().__init__()
         self.fc = nn.Linear(in_channels, out_channels, bias=bias)
         self.nonlinear = nonlinear
@@ -72,8 +110,11 @@ class FullyConnectBlock(nn.Module):
             self._slope = float(nonlinear.negative_slope)
         else:
             raise NotImplementedError("fused epilogue supports LeakyReLU or None")
+        self.norm = LayerNorm(out_channels, negative_slope=self._slope) if layernorm else None
 
     def forward(self, x):
+        if self.norm is not None:
+            return self.norm(LinearFn.apply(x, self.fc.weight, self.fc.bias, 1.0))
         return LinearFn.apply(x, self.fc.weight, self.fc.bias, self._slope)
 
 

@@ -65,6 +65,12 @@ class model(nn.Module):
         self.bilinear = Bilinear(zero_boundary=True, using_scale=True)
         self.strides = [1, 2, 2, 2, 2, 2]
         last = len(enc_filters) - 1
+        # optional (non-reference) key "norm" (default None): "layer" puts a layer norm in front of every LeakyReLU of the encoder
+        # (over a voxel's channels) and of the head (over the features).  The conv blocks then run one by one in plain
+        # channels-last: the fused first pair and the parity-split rows have the LeakyReLU in their epilogues.
+        self.norm = _opt(opt, "norm", None)
+        if self.norm not in (None, "layer"):
+            raise ValueError('norm must be None or "layer"')
         for i, f in enumerate(enc_filters):
             cin = self.drr_feature_num + 1 if i == 0 else enc_filters[i - 1]
             # activations between blocks are channels-last; when a block's output H is even it is written
@@ -73,14 +79,18 @@ class model(nn.Module):
             h_out = _out_size(self.img_sz[2], self.strides[:i + 1])
             lay_in = ops.LAYOUT_NCDHW if i == 0 else (ops.LAYOUT_NDHWC_HPS if h_in % 2 == 0 else ops.LAYOUT_NDHWC)
             lay_out = ops.LAYOUT_NCDHW if i == last else (ops.LAYOUT_NDHWC_HPS if h_out % 2 == 0 else ops.LAYOUT_NDHWC)
+            if self.norm:
+                lay_in, lay_out = (ops.LAYOUT_NDHWC if lay == ops.LAYOUT_NDHWC_HPS else lay for lay in (lay_in, lay_out))
             self.encoders.append(convBlock(cin, f, stride=self.strides[i], bias=True, in_layout=lay_in,
-                                           out_layout=lay_out))
+                                           out_layout=lay_out, layernorm=bool(self.norm)))
         # optional (non-reference) key "conv_dtype": "bf16" stores the activations between the blocks as bfloat16
         # and runs the blocks on the bf16 MFMA (BASELINE configs C4/C5); training computes fp32 gradients of that
         # bf16-forward arithmetic (autograd.EncoderBf16Fn); default "fp32"
         self.conv_dtype = str(_opt(opt, "conv_dtype", "fp32"))
         if self.conv_dtype not in ("fp32", "bf16"):
             raise ValueError('conv_dtype must be "fp32" or "bf16"')
+        if self.norm and self.conv_dtype != "fp32":
+            raise ValueError('norm needs conv_dtype "fp32": the bf16 encoder\'s blocks carry the LeakyReLU in their epilogues')
         # with conv_dtype "bf16": "grad_dtype": "bf16" also stores the pre-activation gradients between the blocks
         # as bf16 (data gradient on the bf16 MFMA); default "fp32" = the exact gradient of the bf16 forward
         self.grad_dtype = str(_opt(opt, "grad_dtype", "fp32"))
@@ -106,8 +116,8 @@ class model(nn.Module):
         flat = enc_filters[-1] * int(np.prod([_out_size(n, self.strides) for n in self.img_sz]))
         self.encoders.append(nn.Sequential(
             nn.Flatten(),
-            FullyConnectBlock(flat, 800),
-            FullyConnectBlock(800, 256),
+            FullyConnectBlock(flat, 800, layernorm=bool(self.norm)),
+            FullyConnectBlock(800, 256, layernorm=bool(self.norm)),
             FullyConnectBlock(256, self.latent_dim, nonlinear=None)))
 
         # PCA basis: kept as the (L, 3V) C-contiguous array of pca_vectors.npy; the reference's
@@ -148,6 +158,8 @@ class model(nn.Module):
         # EXPERIMENTAL since round 6: the kernel is only in the `make exp` build of the library (include/liftreg_hip.h, last
         # section; LIFTREG_HIP_LIB selects it) — asking for it on the product library is an error, not a silent two-kernel run.
         self.fuse_backproject = bool(_opt(opt, "fuse_backproject", False))
+        if self.fuse_backproject and self.norm:
+            raise ValueError("fuse_backproject and norm exclude each other: the fused block has the LeakyReLU in its epilogue")
         if self.fuse_backproject and not _hip.has_experimental():
             raise _hip.LiftRegHipError("fuse_backproject needs the experimental build of libliftreg_hip (make -C liftreg_amd/csrc exp; "
                                        "LIFTREG_HIP_LIB=<libliftreg_hip_exp.so>)")
@@ -367,6 +379,13 @@ class model(nn.Module):
             p = poses.detach().cpu().numpy() if isinstance(poses, torch.Tensor) else np.asarray(poses)
             self._poses = np.ascontiguousarray(p[0], dtype=np.float32)  # poses[0:1] (:87)
         V = D * W * H
+        if self.norm:
+            x = torch.empty((B, P + 1, D, W, H), dtype=torch.float32, device=moving.device)
+            x[:, 0:1].copy_(moving)
+            ops.backproject(target_proj, self._poses, (D, W, H), out=x[:, 1:], out_batch_stride=(P + 1) * V)
+            for i in range(6):
+                x = self.encoders[i](x, packed=self._packed_weight(i))
+            return self.encoders[6](x)
         needs_grad = torch.is_grad_enabled() and any(p.requires_grad for p in self.parameters())
         if self.conv_dtype != "bf16" and not needs_grad and P <= self.PAIR01_MAX_VIEWS:
             # inference, fp32: the first block reads `moving` and the backprojected views from their own buffers —

@@ -777,6 +777,54 @@ def linear_lrelu(x, weight, bias, negative_slope=1.0):
     return y
 
 
+# ----------------------------------------------------------------------------- layer norm
+def _norm_args(x, weight, bias, eps):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x: expected a torch.Tensor, got {type(x).__name__}")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"x: expected float32 or bfloat16, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must have a last axis to normalise, got shape {tuple(x.shape)}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    x = _dev(x, "x", x.dtype)
+    wb = []
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            t = _dev(t.detach(), name)
+            if tuple(t.shape) != (x.shape[-1],) or t.device != x.device:
+                raise ValueError(f"{name} must have shape ({x.shape[-1]},) on {x.device}, got {tuple(t.shape)} on {t.device}")
+        wb.append(t)
+    return x, wb[0], wb[1]
+
+
+def layer_norm(x, weight=None, bias=None, *, eps=1e-5, negative_slope=1.0, return_stats=False):
+    """LeakyReLU(layer norm of x over its last axis * weight + bias), one pass (negative_slope = 1: no activation).
+    x: (..., C) float32 or bfloat16, any number of rows; weight, bias: (C,) float32 or None; y in x's type, statistics in float32.
+    return_stats: (y, stats) for ops_bwd.layer_norm_bwd: a (rows, 2) tensor of mean and 1 / sqrt(var + eps), or None for rows of
+    at most lr_layer_norm_resident_cols() columns, whose backward pass recomputes them from the row it holds in registers."""
+    x, w, b = _norm_args(x, weight, bias, eps)
+    if x.get_device() != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return layer_norm(x, w, b, eps=eps, negative_slope=negative_slope, return_stats=return_stats)
+    lib = _hip.lib()
+    C = x.shape[-1]
+    rows = x.numel() // C
+    y = torch.empty_like(x)
+    stats = ws = None
+    need = lib.lr_layer_norm_workspace(rows, C, 0)
+    if need < 0:
+        _hip.check(int(need), "lr_layer_norm_workspace")
+    if need:
+        ws = torch.empty((need,), dtype=torch.uint8, device=x.device)
+    if return_stats and C > lib.lr_layer_norm_resident_cols():
+        stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
+    with _timed(f"layer_norm_{C}", bytes=2 * x.numel() * x.element_size()):
+        _hip.check(lib.lr_layer_norm(x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(stats), _ptr(ws), rows, C,
+                                     x.dtype == torch.bfloat16, float(eps), float(negative_slope), _stream()), "lr_layer_norm")
+    return (y, stats) if return_stats else y
+
+
 # ----------------------------------------------------------------------------- K5 PCA
 def pca_reconstruct(coefs, basis_LxM, mean, *, out=None):
     """disp (B,M) = coefs (B,L) @ basis (L,M) + mean (M).  Replaces F.linear at …Backproj.py:102.

@@ -1,0 +1,325 @@
+"""The update of the parameters on the HIP kernels (liftreg_amd/csrc/optim.hip): the AdamW step over all the tensors of a model
+in one launch, its states in 32 bits or in block-scaled 8 bits, and the global norm of the gradients that it clips by.
+
+The reference trains with `torch.optim.Adam(eps=1e-5)` (src/liftreg/networks/RegistrationNet.py:245), which `AdamW` with
+`weight_decay=0` is.  GPU tensors only; launches go to torch's current stream of the tensors' device.
+"""
+import array
+import operator
+
+import torch
+
+from . import _hip
+from .ops import _stream, _timed
+
+BLOCK = 32                              # consecutive elements that share a scale in the 8-bit states
+_T = torch.Tensor
+_dtype = operator.attrgetter("dtype")
+
+
+def _column(tensors, name, dtype, device, sizes):
+    """The addresses of a list of tensors, after its checks."""
+    if len(tensors) != len(sizes):
+        raise ValueError(f"{name}: {len(tensors)} tensors for {len(sizes)} parameters")
+    for t in tensors:
+        if not isinstance(t, _T):
+            raise TypeError(f"{name}: expected torch.Tensors, got {type(t).__name__}")
+    where = set(map(_T.get_device, tensors))
+    if where != {device}:
+        if -1 in where:
+            raise _hip.LiftRegHipError(f"{name}: a tensor is on the CPU; liftreg_amd ops run on the GPU only (no CPU fallback)")
+        raise ValueError(f"{name}: all tensors must be on the parameters' device, cuda:{device}")
+    kinds = set(map(_dtype, tensors))
+    if kinds != {dtype}:
+        raise TypeError(f"{name}: expected {dtype}, got {', '.join(sorted(map(str, kinds)))}")
+    if list(map(_T.numel, tensors)) != sizes:
+        raise ValueError(f"{name}: the tensors' sizes do not match the parameters'")
+    if not all(map(_T.is_contiguous, tensors)):
+        raise ValueError(f"{name}: tensors must be contiguous")
+    return list(map(_T.data_ptr, tensors))
+
+
+def _first(tensors, name):
+    tensors = list(tensors)
+    if not tensors:
+        raise ValueError(f"{name}: no tensors")
+    t = tensors[0]
+    if not isinstance(t, _T):
+        raise TypeError(f"{name}: expected torch.Tensors, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise _hip.LiftRegHipError(f"{name}: tensor is on {t.device}; liftreg_amd ops run on the GPU only (no CPU fallback)")
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
+    for u in tensors:
+        if not isinstance(u, _T):
+            raise TypeError(f"{name}: expected torch.Tensors, got {type(u).__name__}")
+    return tensors, t.dtype, t.get_device(), list(map(_T.numel, tensors))
+
+
+def _scalar(x, dtype, device, name):
+    """(value, device address) of a number, or of a one-element tensor that stays on the device."""
+    if not isinstance(x, _T):
+        return x, None
+    if x.dtype != dtype or x.numel() != 1 or x.get_device() != device:
+        raise ValueError(f"{name}: a tensor must be one {dtype} on cuda:{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    return 1, x.data_ptr()
+
+
+def grad_norm(grads):
+    """The 2-norm of all `grads` together (0-dim float32 tensor): fp64 sums in a fixed order, two launches, no synchronisation.
+    grads: float32 or bfloat16 GPU tensors of one type and device, any shapes."""
+    grads, dtype, device, sizes = _first(grads, "grads")
+    with torch.cuda.device(device):
+        addr = _column(grads, "grads", dtype, device, sizes)
+        n = len(sizes)
+        host = array.array("Q", addr + sizes)
+        at = host.buffer_info()[0]
+        lib = _hip.lib()
+        parts = lib.lr_grad_norm_partials(at + 8 * n, n)
+        if parts < 0:
+            _hip.check(int(parts), "lr_grad_norm_partials")
+        partial = torch.empty((max(1, parts),), dtype=torch.float64, device=grads[0].device)
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        with _timed("grad_norm", bytes=sum(sizes) * dtype.itemsize):
+            _hip.check(lib.lr_grad_norm(at, at + 8 * n, n, dtype == torch.bfloat16, partial.data_ptr(), out.data_ptr(), _stream()),
+                       "lr_grad_norm")
+    return out
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
+               grad_norm=None, exp_avg_scales=None, exp_avg_sq_scales=None, seed=0):
+    """One AdamW step over lists of tensors, in place:
+
+        g = grad c,  m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+
+    params, grads: contiguous float32 or bfloat16 tensors (one type; bfloat16 parameters are rounded to nearest — where lr times
+    the update is below 2^-9 of a parameter it no longer moves: keep those in float32).  No tensor may occur twice.
+    exp_avgs, exp_avg_sqs: float32, of the parameters' sizes; or, with exp_avg_scales and exp_avg_sq_scales, block-scaled 8-bit
+    states: float8_e4m3fn / float8_e5m2 codes of the parameters' sizes and one float8_e8m0fnu scale for each 32 consecutive
+    elements (`state8` makes them, `values8` reads them).  They are rounded stochastically: the random bits are a function of
+    (seed, step, position of the element in the call's tensors), so equal calls give equal bits.  A block with an element that is
+    not finite becomes NaN as a whole.
+    step: 1 for the first step; lr: both numbers, or one-element device tensors (int64, float32) that a captured graph reads
+    at each replay.
+    max_norm: the gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in (they are not written); norm is
+    `grad_norm` (0-dim float32 tensor) or, if that is None, the 2-norm of all of `grads`, computed here.  A norm that is not finite
+    reaches the parameters.  Returns the norm (0-dim float32 tensor), None without max_norm."""
+    params, dtype, device, sizes = _first(params, "params")
+    grads, exp_avgs, exp_avg_sqs = list(grads), list(exp_avgs), list(exp_avg_sqs)
+    b1, b2 = betas
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+        raise ValueError(f"betas must be in [0, 1), eps and weight_decay not negative; got {betas}, {eps}, {weight_decay}")
+    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
+        raise ValueError("8-bit states need both exp_avg_scales and exp_avg_sq_scales")
+    if max_norm is None and grad_norm is not None:
+        raise ValueError("grad_norm is for max_norm")
+    if max_norm is not None and not max_norm > 0.0:
+        raise ValueError(f"max_norm must be positive, got {max_norm}")
+    eight = exp_avg_scales is not None
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return adamw_step(params, grads, exp_avgs, exp_avg_sqs, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                              max_norm=max_norm, grad_norm=grad_norm, exp_avg_scales=exp_avg_scales,
+                              exp_avg_sq_scales=exp_avg_sq_scales, seed=seed)
+    n = len(sizes)
+    p = _column(params, "params", dtype, device, sizes)
+    m = _column(exp_avgs, "exp_avgs", torch.float8_e4m3fn if eight else torch.float32, device, sizes)
+    v = _column(exp_avg_sqs, "exp_avg_sqs", torch.float8_e5m2 if eight else torch.float32, device, sizes)
+    scales = []
+    if eight:
+        blocks = [-(-k // BLOCK) for k in sizes]
+        scales = (_column(list(exp_avg_scales), "exp_avg_scales", torch.float8_e8m0fnu, device, blocks) +
+                  _column(list(exp_avg_sq_scales), "exp_avg_sq_scales", torch.float8_e8m0fnu, device, blocks))
+    g = _column(grads, "grads", dtype, device, sizes)
+    written = [a for a in p + m + v + scales if a]
+    if len(set(written)) != len(written):
+        raise ValueError("a parameter or state occurs twice in the call")
+    lr, lr_dev = _scalar(lr, torch.float32, device, "lr")
+    step, step_dev = _scalar(step, torch.int64, device, "step")
+    if lr < 0.0 or step < 1:
+        raise ValueError(f"lr must not be negative and step starts at 1; got {lr}, {step}")
+    host = array.array("Q", p + g + m + v + scales + sizes)
+    at = host.buffer_info()[0]
+    col = [at + 8 * n * k for k in range(7)]
+    numel = col[6] if eight else col[4]
+    lib = _hip.lib()
+    norm, norm_in, partial, out = None, None, None, None
+    if max_norm is not None:
+        norm = grad_norm
+        if norm is None:
+            parts = lib.lr_grad_norm_partials(numel, n)
+            if parts < 0:
+                _hip.check(int(parts), "lr_grad_norm_partials")
+            partial = torch.empty((max(1, parts),), dtype=torch.float64, device=params[0].device)
+            norm = torch.empty((), dtype=torch.float32, device=params[0].device)
+            out = norm.data_ptr()
+        else:
+            norm_in = _scalar(norm, torch.float32, device, "grad_norm")[1]
+            if norm_in is None:
+                raise TypeError("grad_norm: expected a 0-dim float32 tensor")
+    total = sum(sizes)
+    with _timed("adamw_step", bytes=total * (3 * dtype.itemsize + (4 if eight else 16))):
+        _hip.check(lib.lr_adamw_step(col[0], col[1], col[2], col[3], col[4] if eight else None, col[5] if eight else None, numel, n,
+                                     dtype == torch.bfloat16, lr, b1, b2, eps, weight_decay, step, lr_dev, step_dev, max_norm or 0.0,
+                                     norm_in, None if partial is None else partial.data_ptr(), out, seed & 0xFFFFFFFFFFFFFFFF,
+                                     _stream()), "lr_adamw_step")
+    torch.autograd.graph.increment_version(params)     # written behind autograd's back: caches keyed on the version see it
+    return norm
+
+
+def state8(p):
+    """(codes e4m3, scales, codes e5m2, scales): the 8-bit states of parameter `p`, at zero."""
+    def zeros(shape, dtype):
+        return torch.zeros(shape, dtype=torch.uint8, device=p.device).view(dtype)
+
+    blocks = (-(-p.numel() // BLOCK),)
+    return (zeros(p.shape, torch.float8_e4m3fn), zeros(blocks, torch.float8_e8m0fnu), zeros(p.shape, torch.float8_e5m2),
+            zeros(blocks, torch.float8_e8m0fnu))
+
+
+def values8(codes, scales):
+    """The float32 values that 8-bit states stand for: code * scale of its block of 32 consecutive elements."""
+    s = scales.to(torch.float32).repeat_interleave(BLOCK)[:codes.numel()]
+    return codes.to(torch.float32) * s.view(codes.shape)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW on the kernel above, in torch.optim's manner: parameter groups, closures, LR schedulers, state_dict (32-bit states
+    have the keys of torch.optim.Adam / AdamW, whose checkpoints load).  `weight_decay=0` is Adam, the reference's optimizer.
+
+        opt = AdamW(net.parameters(), lr=1e-4, eps=1e-5, weight_decay=0.0, max_grad_norm=1.0)
+
+    state_bits: 32, or 8 for block-scaled 8-bit states (2.06 bytes an element instead of 8).
+    max_grad_norm: clip the 2-norm of all gradients, inside the step; `opt.grad_norm` is the last step's norm (0-dim tensor).
+    seed: of the stochastic rounding of 8-bit states.
+    capturable: the step count lives on the device (int64 tensor), so that `step()` can be captured in a graph; the groups'
+    "lr" may then be a one-element float32 device tensor, which a replay reads.  A replay does not run Python: call the model's
+    `invalidate_packed()` before inference with parameters that replays have changed.
+    Parameters: contiguous float32 or bfloat16 GPU tensors; gradients of the parameter's type, dense."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None, seed=0,
+                 capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not max_grad_norm > 0.0:
+            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
+        self.state_bits, self.max_grad_norm, self.seed, self.capturable = state_bits, max_grad_norm, int(seed), bool(capturable)
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        b1, b2 = group.get("betas", self.defaults["betas"])
+        lr = group.get("lr", self.defaults["lr"])
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not lr >= 0.0 or group.get("eps", self.defaults["eps"]) < 0.0 or \
+                group.get("weight_decay", self.defaults["weight_decay"]) < 0.0:
+            raise ValueError("betas must be in [0, 1), lr, eps and weight_decay not negative")
+        if isinstance(lr, _T) and lr.is_cuda and not self.capturable:
+            raise ValueError("a learning rate on the device needs capturable=True")
+        super().add_param_group(group)
+
+    def _new_state(self, p, steps):
+        if self.state_bits == 8:
+            m, ms, v, vs = state8(p)
+            s = {"exp_avg": m, "exp_avg_scale": ms, "exp_avg_sq": v, "exp_avg_sq_scale": vs}
+        else:
+            s = {"exp_avg": torch.zeros(p.shape, dtype=torch.float32, device=p.device),
+                 "exp_avg_sq": torch.zeros(p.shape, dtype=torch.float32, device=p.device)}
+        if self.capturable:          # parameters that start together share their count
+            if p.device not in steps:
+                steps[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+            return {"step": steps[p.device], **s}
+        return {"step": 0, **s}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls, steps = {}, {}
+        for gi, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise ValueError("sparse gradients are not supported")
+                if g.dtype != p.dtype:
+                    raise TypeError(f"gradient is {g.dtype}, its parameter {p.dtype}")
+                s = self.state[p]
+                if not s:
+                    s.update(self._new_state(p, steps))
+                # one call for the parameters of a group that have one type, device and step count
+                t = s["step"]
+                key = (gi, p.dtype, p.device, id(t) if isinstance(t, _T) else t)
+                if key not in calls:
+                    calls[key] = ([], [], [])
+                ps, gs, ss = calls[key]
+                ps.append(p)
+                gs.append(g if g.is_contiguous() else g.contiguous())
+                ss.append(s)
+        self.grad_norm = None
+        norm = None
+        if self.max_grad_norm is not None and len(calls) > 1:
+            kinds = {}
+            for (_, dtype, device, _), (_, gs, _) in calls.items():
+                kinds.setdefault((dtype, device), []).extend(gs)
+            if len({device for _, device in kinds}) > 1:
+                raise ValueError("max_grad_norm: all parameters must be on one device")
+            norms = [grad_norm(gs) for gs in kinds.values()]
+            norm = norms[0] if len(norms) == 1 else grad_norm([torch.stack(norms)])
+        counted = set()
+        for (gi, _, _, _), (ps, gs, ss) in calls.items():
+            group = self.param_groups[gi]
+            t = ss[0]["step"]
+            if isinstance(t, _T):
+                if id(t) not in counted:      # shared by several calls: counted once
+                    counted.add(id(t))
+                    t.add_(1)
+            else:
+                t += 1
+                for s in ss:
+                    s["step"] = t
+            lr = group["lr"]
+            if isinstance(lr, _T) and not lr.is_cuda:
+                lr = float(lr)
+            eight = self.state_bits == 8
+            out = adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], step=t, lr=lr, betas=group["betas"],
+                             eps=group["eps"], weight_decay=group["weight_decay"], max_norm=self.max_grad_norm, grad_norm=norm,
+                             exp_avg_scales=[s["exp_avg_scale"] for s in ss] if eight else None,
+                             exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in ss] if eight else None,
+                             seed=self.seed + (gi << 32))      # groups draw different bits
+            self.grad_norm = out
+        return loss
+
+    @torch.no_grad()
+    def load_state_dict(self, state_dict):
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("amsgrad and maximize are not built")
+        want = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
+        for s in state_dict["state"].values():
+            if set(s) - {"step"} != want:
+                raise ValueError(f"the checkpoint's states {sorted(s)} are not those of state_bits={self.state_bits}")
+        super().load_state_dict(state_dict)
+        # the base class casts every state to its parameter's type: take the checkpoint's own values again
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        ours = [p for g in self.param_groups for p in g["params"]]
+        like = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}[self.state_bits]
+        shared = {}
+        for i, p in zip(ids, ours):
+            if i not in state_dict["state"]:
+                continue
+            src, t = state_dict["state"][i], int(state_dict["state"][i]["step"])
+            for k, dtype in zip(("exp_avg", "exp_avg_sq"), like):
+                if tuple(src[k].shape) != tuple(p.shape) or src[k].dtype != dtype:
+                    raise ValueError(f"the checkpoint's {k} is {src[k].dtype} {tuple(src[k].shape)}, needed: {dtype} {tuple(p.shape)}")
+            if self.capturable:
+                if (p.device, t) not in shared:
+                    shared[p.device, t] = torch.tensor(t, dtype=torch.int64, device=p.device)
+                t = shared[p.device, t]
+            self.state[p] = {"step": t, **{k: src[k].detach().to(device=p.device, copy=True).contiguous() for k in sorted(want)}}
+        for group in self.param_groups:
+            for k, v in self.defaults.items():
+                group.setdefault(k, v)

@@ -303,6 +303,8 @@ class SlabShardedRegistration:
     GATHER_DEPTH = 32      # all-gather the activation behind the first block with at most this many output planes
 
     def __init__(self, net, comm, sim_variant=NCC_CONFIGURED):
+        if getattr(net, "norm", None):
+            raise ValueError("slab sharding walks the encoder's conv kernels itself: a model with norm is not built for it")
         self.net, self.comm, self.variant = net, comm, sim_variant
         D = net.img_sz[0]
         need = self.slab_multiple(net) * comm.world

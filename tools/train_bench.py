@@ -92,6 +92,9 @@ def main():
     ap.add_argument("--no-kernel-table", action="store_true")
     ap.add_argument("--model-opt", action="append", default=[], metavar="KEY=BOOL",
                     help="a boolean model option, e.g. reg_in_coef_space=false ncc_grad_via_moments=false (A/B aid)")
+    ap.add_argument("--optimizer", default="torch", choices=("torch", "hip32", "hip8"),
+                    help="torch: torch.optim.Adam; hip32 / hip8: liftreg_amd.optim.AdamW(weight_decay=0) with 32-bit / 8-bit states")
+    ap.add_argument("--norm", default=None, choices=("layer",), help="layer: the model option norm (layer norm in encoder and head)")
     ap.add_argument("--adam-foreach", action="store_true", help="torch's default (multi-pass) Adam instead of fused=True (A/B aid)")
     ap.add_argument("--dry-run", action="store_true", help="CPU/gloo control-path self-test with a stand-in module")
     ap.add_argument("--batch", type=int, default=None, help="registrations per rank (default: the configuration's)")
@@ -160,7 +163,7 @@ def main():
         from liftreg_amd.utils.sdct_projection_utils import scan_poses
         net = model([n, n, n], {"drr_feature_num": P, "latent_dim": L, "pca_path": "synthetic:2021",
                                 "conv_dtype": a.conv_dtype, "grad_dtype": a.grad_dtype,
-                                "pca_dtype": a.pca_dtype,
+                                "pca_dtype": a.pca_dtype, "norm": a.norm,
                                 **{k: (v.lower() in ("1", "true", "yes")) for k, v in (kv.split("=", 1) for kv in a.model_opt)}}).to(dev).train()
         crit = SubspaceLoss({"initial_reg_factor": 0.01, "min_reg_factor": 0.01, "reg_factor_decay_from": 2})
         crit.sim.check_nan = False
@@ -182,7 +185,11 @@ def main():
 
     # RegistrationNet.py:245 (Adam, eps 1e-5).  fused=True is torch's own single-kernel implementation of the same update
     # (one pass over p, g, m, v instead of the default's ~8 elementwise passes); --adam-foreach selects the default
-    opt = torch.optim.Adam(net.parameters(), lr=1e-4, eps=1e-5, **({} if (a.adam_foreach or a.dry_run) else {"fused": True}))
+    if a.optimizer == "torch" or a.dry_run:
+        opt = torch.optim.Adam(net.parameters(), lr=1e-4, eps=1e-5, **({} if (a.adam_foreach or a.dry_run) else {"fused": True}))
+    else:
+        from liftreg_amd.optim import AdamW
+        opt = AdamW(net.parameters(), lr=1e-4, eps=1e-5, weight_decay=0.0, state_bits=int(a.optimizer[3:]))
     ddp = GradientAllReduce(net) if (world > 1 or a.ddp) else None
 
     def step(ep):
