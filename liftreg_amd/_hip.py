@@ -157,6 +157,24 @@ def lib():
     return _lib
 
 
+_tensors = None
+
+
+def tensors():
+    """liblr_tensors.so (csrc/tensors.cpp): lr_gather_tensors, the checks and addresses of lists of tensors in one call."""
+    global _tensors
+    if _tensors is None:
+        path = os.path.join(CSRC, "liblr_tensors.so")
+        if not os.path.exists(path):
+            raise LiftRegHipError(f"{path} not found: build it with `make -C liftreg_amd/csrc`")
+        import torch  # noqa: F401  (its libraries resolve the symbols)
+        handle = C.PyDLL(path)
+        fn = handle.lr_gather_tensors
+        fn.restype, fn.argtypes = _i64, [C.py_object, C.c_char_p, _i, _p, _i64, _p]
+        _tensors = handle
+    return _tensors
+
+
 def has_experimental():
     """True when the loaded library is the experimental build (include/liftreg_hip.h, last section)."""
     return all(hasattr(lib(), n) for n in EXPERIMENTAL_SIGNATURES)

@@ -19,7 +19,6 @@ namespace {
 
 constexpr int kResident = 16384;       // longest row that is held in registers: 1024 lanes of 16 elements
 constexpr int kBlocks = 2048;          // workgroups of the resident kernels: eight of four waves on each of 256 CUs
-constexpr int kFinish = 32;            // columns of a workgroup that adds partial rows
 
 template <class T> struct Vec;
 template <> struct Vec<float> {
@@ -40,20 +39,44 @@ template <> struct Vec<uint16_t> {     // bfloat16
 };
 
 // N elements from column c of a row of C (past the end: 0, not written).  A row may start at any element: gfx950 takes 16-byte
-// accesses at any address.
-template <class T>
+// accesses at any address.  RAGGED = false: C is a multiple of N.  The last, partial vector of a ragged row is loaded element by
+// element or, SHIFT, as the row's last N elements, shifted down.  Measured backward, where the row's two loads feed three dependent
+// sums: bf16 (7 elements at worst) 44739 x 1500 209 us by element, 163 shifted; fp32 (3 at worst) 22362 x 3001 181 and 222.
+__device__ __forceinline__ void shifted(const uint16_t* row, int64_t c, int64_t C, float* r) {
+  typedef uint64_t Q __attribute__((ext_vector_type(2), aligned(2)));
+  const int64_t at = C - 8;
+  const Q t = *reinterpret_cast<const Q*>(row + (c < at ? c : at));
+  const int d = c < at ? 0 : (int)min(c - at, (int64_t)8);
+  const int n = 16 * (d & 3);
+  uint64_t lo = d & 4 ? t[1] : t[0], hi = d & 4 ? 0 : t[1];
+  lo = n ? lo >> n | hi << (64 - n) : lo;
+  hi >>= n;
+  if (d >= 8) lo = hi = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    r[e] = Vec<uint16_t>::up((uint16_t)(lo >> (16 * e)));
+    r[e + 4] = Vec<uint16_t>::up((uint16_t)(hi >> (16 * e)));
+  }
+}
+template <bool RAGGED = true, bool SHIFT = false, class T>
 __device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* r) {
   constexpr int N = Vec<T>::N;
-  if (c + N <= C) {
+  if constexpr (RAGGED && SHIFT) {
+    if (C >= N) {
+      shifted(row, c, C, r);
+      return;
+    }
+  }
+  if (RAGGED ? c + N <= C : c < C) {
     const typename Vec<T>::V v = *reinterpret_cast<const typename Vec<T>::V*>(row + c);
 #pragma unroll
     for (int e = 0; e < N; ++e) r[e] = Vec<T>::up(v[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = c + e < C ? Vec<T>::up(row[c + e]) : 0.f;
+    for (int e = 0; e < N; ++e) r[e] = RAGGED && c + e < C ? Vec<T>::up(row[c + e]) : 0.f;
   }
 }
-template <class T>
+template <bool RAGGED = true, class T>
 __device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float* r) {
   constexpr int N = Vec<T>::N;
   if (c + N <= C) {
@@ -61,7 +84,7 @@ __device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float*
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = Vec<T>::down(r[e]);
     *reinterpret_cast<typename Vec<T>::V*>(row + c) = v;
-  } else {
+  } else if (RAGGED) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
       if (c + e < C) row[c + e] = Vec<T>::down(r[e]);
@@ -74,7 +97,7 @@ __device__ __forceinline__ void load_f(const float* a, int64_t c, int64_t C, flo
   if (!a) return;
   if (c + N <= C) {
 #pragma unroll
-    for (int q = 0; q < N; q += 4) load(a, c + q, C, r + q);
+    for (int q = 0; q < N; q += 4) load<false>(a, c + q, C, r + q);
   } else {
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -101,24 +124,35 @@ __device__ __forceinline__ float lane_sum(float x) {
 // sums over the G lanes of a row.  Above a wave: through LDS, two buffers in turn, one barrier a sum.
 template <int G, int NT>
 struct Group {
-  float (*red)[NT / 64];
+  static constexpr int W = G / 64;       // waves of a row
+  float (*red)[2][NT / 64];
   int turn;
-  __device__ __forceinline__ explicit Group(float (*r)[NT / 64]) : red(r), turn(0) {}
+  __device__ __forceinline__ explicit Group(float (*r)[2][NT / 64]) : red(r), turn(0) {}
   __device__ __forceinline__ float sum(float x) {
     if (G <= 64) return lane_sum<G>(x);
-    x = lane_sum<64>(x);
-    float* buf = red[turn];
-    turn ^= 1;
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = x;
-    __syncthreads();
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) s += buf[w];
-    return s;
+    float y = 0.f;
+    sum2(x, y);
+    return x;
   }
   __device__ __forceinline__ void sum2(float& a, float& b) {
-    a = sum(a);
-    b = sum(b);
+    a = lane_sum<(G < 64 ? G : 64)>(a);
+    b = lane_sum<(G < 64 ? G : 64)>(b);
+    if (G <= 64) return;
+    float (*buf)[NT / 64] = red[turn];
+    turn ^= 1;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      buf[0][wave] = a;
+      buf[1][wave] = b;
+    }
+    __syncthreads();
+    const int first = W > 0 ? wave / (W > 0 ? W : 1) * W : 0;
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      a += buf[0][first + w];
+      b += buf[1][first + w];
+    }
   }
 };
 
@@ -151,7 +185,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
                                                  T* __restrict__ y, float* __restrict__ stats, int64_t rows, int C, float inv,
                                                  float eps, float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G;
-  __shared__ float red[2][NT / 64];
+  __shared__ float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
   float wv[K * N], bv[K * N];
@@ -166,7 +200,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
     const T* xr = x + r * C;
     float v[K * N];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load(xr, (k * G + lane) * N, cols, v + k * N);
+    for (int k = 0; k < K; ++k) load<RAGGED>(xr, (k * G + lane) * N, cols, v + k * N);
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
 #pragma unroll
@@ -176,7 +210,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
         const float z = fmaf((v[k * N + e] - mean) * rstd, wv[k * N + e], bv[k * N + e]);
         v[k * N + e] = z >= 0.f ? z : z * slope;
       }
-      store(y + r * C, (k * G + lane) * N, cols, v + k * N);
+      store<RAGGED>(y + r * C, (k * G + lane) * N, cols, v + k * N);
     }
     if (stats && lane == 0 && r < rows) {
       stats[2 * r] = mean;
@@ -185,31 +219,54 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
   }
 }
 
-// gx (if set) and, where `part` is set, this workgroup's sums of g xhat and g in part[blockIdx.x][2][C]
-template <class T, int G, int K, int NT, bool RAGGED>
+// gx (if set), and this workgroup's sums of g xhat and g at sw, sb (if set) + blockIdx.x * stride.  ACT: there is a LeakyReLU mask
+// (without it b is not needed: 16 of 112 registers at 16 elements a lane).  The next rows are loaded before this round's sums
+// (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.
+template <class T, int G, int K, int NT, bool RAGGED, bool ACT>
 __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
-                                                 const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ part, int64_t rows,
-                                                 int C, float inv, float eps, float slope) {
+                                                 const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ sw, float* __restrict__ sb,
+                                                 int64_t stride, int64_t rows, int C, float inv, float eps, float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G, E = K * N;
-  __shared__ float red[2][NT / 64];
+  constexpr bool AHEAD = E <= 8;
+  __shared__ float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
-  float wv[E], bv[E], aw[E], ab[E];
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  float wv[E], bv[ACT ? E : 1], aw[E], ab[E], v[E], g[E], nv[AHEAD ? E : 1], ng[AHEAD ? E : 1];
+  int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
+  if (AHEAD) {
+    const int cols = r < rows ? C : 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + r * C, (k * G + lane) * N, cols, (AHEAD ? nv : v) + k * N);
+#pragma unroll
+    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + r * C, (k * G + lane) * N, cols, (AHEAD ? ng : g) + k * N);
+  }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     load_f<N>(w, (k * G + lane) * N, C, 1.f, wv + k * N);
-    load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + k * N);
+    if (ACT) load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + (ACT ? k * N : 0));
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
-  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += (int64_t)gridDim.x * RPB) {
-    const int64_t r = r0 + threadIdx.x / G;
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step, r += step) {
     const int cols = r < rows ? C : 0;
-    float v[E], g[E];
+    if (AHEAD) {
+      const int next = r + step < rows ? C : 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) load(x + r * C, (k * G + lane) * N, cols, v + k * N);
+      for (int i = 0; i < E; ++i) {
+        v[i] = nv[AHEAD ? i : 0];
+        g[i] = ng[AHEAD ? i : 0];
+      }
 #pragma unroll
-    for (int k = 0; k < K; ++k) load(gy + r * C, (k * G + lane) * N, cols, g + k * N);
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? nv : v) + k * N);
+#pragma unroll
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? ng : g) + k * N);
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + r * C, (k * G + lane) * N, cols, v + k * N);
+#pragma unroll
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + r * C, (k * G + lane) * N, cols, g + k * N);
+    }
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
     if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
@@ -217,7 +274,8 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
 #pragma unroll
     for (int i = 0; i < E; ++i) {     // past the end g = 0: nothing is added
       const float xh = (v[i] - mean) * rstd;
-      const float gg = fmaf(xh, wv[i], bv[i]) >= 0.f ? g[i] : g[i] * slope;
+      float gg = g[i];
+      if (ACT) gg = fmaf(xh, wv[i], bv[ACT ? i : 0]) >= 0.f ? gg : gg * slope;
       aw[i] = fmaf(gg, xh, aw[i]);
       ab[i] += gg;
       const float h = gg * wv[i];
@@ -237,11 +295,11 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
           const int i = k * N + e;
           v[i] = rstd * (g[i] - fmaf(v[i], s2, s1));
         }
-        store(gx + r * C, (k * G + lane) * N, cols, v + k * N);
+        store<RAGGED>(gx + r * C, (k * G + lane) * N, cols, v + k * N);
       }
     }
   }
-  if (!part) return;
+  if (!sw && !sb) return;
   // groups of a wave, then waves
 #pragma unroll
   for (int i = 0; i < E; ++i)
@@ -249,30 +307,30 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
       aw[i] += __shfl_xor(aw[i], o, 64);
       ab[i] += __shfl_xor(ab[i], o, 64);
     }
-  float* p = part + (int64_t)blockIdx.x * 2 * C;
-  if (G > 64) {
+  const int64_t at0 = (int64_t)blockIdx.x * stride;
+  if (G == NT) {         // one row at a time: every column has one lane
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const int c = (k * G + lane) * N + e;
         if (c < C) {
-          p[c] = aw[k * N + e];
-          p[C + c] = ab[k * N + e];
+          if (sw) sw[at0 + c] = aw[k * N + e];
+          if (sb) sb[at0 + c] = ab[k * N + e];
         }
       }
     return;
   }
-  constexpr int W = G > 64 ? 1 : NT / 64, L = G > 64 ? 1 : G * E;      // waves, columns
+  constexpr int W = G == NT ? 1 : G <= 64 ? NT / 64 : NT / G, L = G == NT ? 1 : G * E;      // sums to add, columns
   __shared__ float cols[W][2][L];
-  const int wave = threadIdx.x >> 6, at = threadIdx.x & 63;
+  const int set = threadIdx.x / (G <= 64 ? 64 : G), at = threadIdx.x % (G <= 64 ? 64 : G);
   if (at < G) {
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        cols[wave % W][0][((k * G + at) * N + e) % L] = aw[k * N + e];
-        cols[wave % W][1][((k * G + at) * N + e) % L] = ab[k * N + e];
+        cols[set % W][0][((k * G + at) * N + e) % L] = aw[k * N + e];
+        cols[set % W][1][((k * G + at) * N + e) % L] = ab[k * N + e];
       }
   }
   __syncthreads();
@@ -280,29 +338,36 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
     const int which = i >= C, c = i - which * C;
     float s = 0.f;
     for (int q = 0; q < W; ++q) s += cols[q][which][c];
-    p[i] = s;
+    float* out = which ? sb : sw;
+    if (out) out[at0 + c] = s;
   }
 }
 
-// out[0..C) = sum of the first half of the partial rows [n][2 C], out2 of the second, in a fixed order
-__global__ __launch_bounds__(1024) void finish_kernel(const float* __restrict__ part, int n, int64_t C, float* __restrict__ gw,
-                                                      float* __restrict__ gb) {
-  __shared__ float red[1024 / kFinish][kFinish + 1];
-  const int64_t c = (int64_t)blockIdx.x * kFinish + threadIdx.x % kFinish;
-  const int j = threadIdx.x / kFinish;
+// gw = sum of the first halves of the partial rows [n][2 C], gb of the second, in a fixed order; LANES rows at a time: 32 where there
+// are many rows, one (a column a thread) where there are few and long ones (2 rows of 1 M: 142 us with 32, 7 with one)
+template <int LANES>
+__global__ __launch_bounds__(LANES == 1 ? 256 : 1024) void finish_kernel(const float* __restrict__ part, int n, int64_t C,
+                                                                         float* __restrict__ gw, float* __restrict__ gb) {
+  constexpr int COLS = LANES == 1 ? 256 : 1024 / LANES;
+  const int64_t c = (int64_t)blockIdx.x * COLS + threadIdx.x % COLS;
+  const int j = threadIdx.x / COLS;
   float s = 0.f;
   if (c < 2 * C)
 #pragma unroll 8
-    for (int i = j; i < n; i += 1024 / kFinish) s += part[(int64_t)i * 2 * C + c];
-  red[j][threadIdx.x % kFinish] = s;
-  __syncthreads();
-  for (int o = 1024 / kFinish / 2; o > 0; o >>= 1) {
-    if (j < o) red[j][threadIdx.x % kFinish] += red[j + o][threadIdx.x % kFinish];
+    for (int i = j; i < n; i += LANES) s += part[(int64_t)i * 2 * C + c];
+  if (LANES > 1) {
+    __shared__ float red[LANES][COLS + 1];
+    red[j][threadIdx.x % COLS] = s;
     __syncthreads();
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      if (j < o) red[j][threadIdx.x % COLS] += red[j + o][threadIdx.x % COLS];
+      __syncthreads();
+    }
+    s = red[0][threadIdx.x % COLS];
   }
   if (j == 0 && c < 2 * C) {
     float* out = c < C ? gw : gb;
-    if (out) out[c < C ? c : c - C] = red[0][threadIdx.x];
+    if (out) out[c < C ? c : c - C] = s;
   }
 }
 
@@ -369,29 +434,43 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ 
   }
 }
 
-// stats[row] from the row's chunks
-__global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ part, int chunks, int64_t C, int64_t len,
-                                                         float eps, float* __restrict__ stats, int64_t row0) {
-  const int64_t row = row0 + blockIdx.x;
+// mean and rstd of a row from its chunks, by a whole workgroup
+__device__ __forceinline__ void join_stats(const float* part, int64_t row, int chunks, int64_t C, int64_t len, float eps, float& mean,
+                                           float& rstd) {
   Part p = {0.f, 0.f, 0.f};
   for (int i = threadIdx.x; i < chunks; i += 256) {
     const float* o = part + (row * chunks + i) * 2;
     p = join(p, {(float)min(len, C - i * len), o[0], o[1]});
   }
   p = block_join(p);
+  mean = p.mean;
+  rstd = 1.0f / sqrtf(p.m2 / (float)C + eps);
+}
+
+__global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ part, int chunks, int64_t C, int64_t len,
+                                                         float eps, float* __restrict__ stats, int64_t row0) {
+  const int64_t row = row0 + blockIdx.x;
+  float mean, rstd;
+  join_stats(part, row, chunks, C, len, eps, mean, rstd);
   if (threadIdx.x == 0) {
-    stats[2 * row] = p.mean;
-    stats[2 * row + 1] = 1.0f / sqrtf(p.m2 / (float)C + eps);
+    stats[2 * row] = mean;
+    stats[2 * row + 1] = rstd;
   }
 }
 
+// every workgroup joins its row's statistics again (at most 8 KB from L2): a launch of its own for them takes 4.6 us
 template <class T>
 __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
-                                                        T* __restrict__ y, const float* __restrict__ stats, int64_t C, int64_t len,
-                                                        float slope, int64_t row0) {
+                                                        T* __restrict__ y, const float* __restrict__ part, float* __restrict__ stats,
+                                                        int64_t C, int64_t len, float eps, float slope, int64_t row0) {
   constexpr int N = Vec<T>::N;
   const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
-  const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+  float mean, rstd;
+  join_stats(part, row, gridDim.x, C, len, eps, mean, rstd);
+  if (stats && blockIdx.x == 0 && threadIdx.x == 0) {
+    stats[2 * row] = mean;
+    stats[2 * row + 1] = rstd;
+  }
 #pragma unroll 4
   for (int64_t c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
     float v[N], wv[N], bv[N];
@@ -408,7 +487,7 @@ __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x,
 }
 
 // sums of h and h xhat over a chunk of a row
-template <class T>
+template <class T, bool ACT>
 __global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                          const T* __restrict__ gy, const float* __restrict__ stats,
                                                          float* __restrict__ part, int64_t C, int64_t len, float slope, int64_t row0) {
@@ -423,12 +502,12 @@ __global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x
     load(x + row * C, c, hi, v);
     load(gy + row * C, c, hi, g);
     load_f<N>(w, c, hi, 1.f, wv);
-    load_f<N>(b, c, hi, 0.f, bv);
+    if (ACT) load_f<N>(b, c, hi, 0.f, bv);
     float t1 = 0.f, t2 = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float xh = (v[e] - mean) * rstd;
-      const float h = (fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope) * wv[e];
+      const float h = (!ACT || fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope) * wv[e];
       t1 += h;
       t2 = c + e < hi ? fmaf(h, xh, t2) : t2;
     }
@@ -469,20 +548,41 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict_
         ((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x])) / (float)C;
 }
 
-// columns of a workgroup, rows [blockIdx.y * span, + span): gx, and the columns' sums over these rows
-template <class T>
+// columns of a workgroup, rows [row0 + blockIdx.y * span, + span) below row1: gx, and the columns' sums over these rows (`more`: on top of
+// what is there).  JOIN: the rows' sums of h and
+// h xhat are added up from their chunks here, a wave a row (span rows of `chunks` chunks, at most kJoin in all); else `sums` holds
+// the means.
+constexpr int kJoin = 2048;
+template <class T, bool JOIN, bool ACT>
 __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                         const T* __restrict__ gy, const float* __restrict__ stats,
                                                         const float* __restrict__ sums, T* __restrict__ gx, float* __restrict__ gw,
-                                                        float* __restrict__ gb, int64_t stride, int64_t rows, int64_t span, int64_t C,
-                                                        float slope) {
+                                                        float* __restrict__ gb, int64_t stride, int64_t row0, int64_t row1, int64_t span,
+                                                        int chunks, int64_t C, float slope, bool more) {
   constexpr int N = Vec<T>::N;
+  __shared__ float joined[JOIN ? kJoin : 1][2];
   const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * N;
-  const int64_t lo = blockIdx.y * span, hi = min(rows, lo + span);
+  const int64_t lo = row0 + blockIdx.y * span, hi = min(row1, lo + span);
+  if (JOIN) {
+    for (int64_t r = lo + (threadIdx.x >> 6); r < hi; r += 4) {
+      float s1 = 0.f, s2 = 0.f;
+      for (int i = threadIdx.x & 63; i < chunks; i += 64) {
+        s1 += sums[(r * chunks + i) * 2];
+        s2 += sums[(r * chunks + i) * 2 + 1];
+      }
+      s1 = lane_sum<64>(s1);
+      s2 = lane_sum<64>(s2);
+      if ((threadIdx.x & 63) == 0) {
+        joined[r - lo][0] = s1 / (float)C;
+        joined[r - lo][1] = s2 / (float)C;
+      }
+    }
+    __syncthreads();
+  }
   if (c >= C) return;
   float wv[N], bv[N], aw[N], ab[N];
   load_f<N>(w, c, C, 1.f, wv);
-  load_f<N>(b, c, C, 0.f, bv);
+  if (ACT) load_f<N>(b, c, C, 0.f, bv);
 #pragma unroll
   for (int e = 0; e < N; ++e) aw[e] = ab[e] = 0.f;
 #pragma unroll 2
@@ -490,11 +590,12 @@ __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x,
     float v[N], g[N];
     load(x + r * C, c, C, v);
     load(gy + r * C, c, C, g);
-    const float mean = stats[2 * r], rstd = stats[2 * r + 1], s1 = sums[2 * r], s2 = sums[2 * r + 1];
+    const float mean = stats[2 * r], rstd = stats[2 * r + 1];
+    const float s1 = JOIN ? joined[r - lo][0] : sums[2 * r], s2 = JOIN ? joined[r - lo][1] : sums[2 * r + 1];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float xh = (v[e] - mean) * rstd;
-      const float gg = fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope;
+      const float gg = !ACT || fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope;
       aw[e] = fmaf(gg, xh, aw[e]);
       ab[e] += gg;
       v[e] = rstd * (gg * wv[e] - fmaf(xh, s2, s1));
@@ -504,46 +605,69 @@ __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x,
 #pragma unroll
   for (int e = 0; e < N; ++e)
     if (c + e < C) {
-      if (gw) gw[blockIdx.y * stride + c + e] = aw[e];
-      if (gb) gb[blockIdx.y * stride + c + e] = ab[e];
+      const int64_t at = blockIdx.y * stride + c + e;
+      if (gw) gw[at] = more ? gw[at] + aw[e] : aw[e];
+      if (gb) gb[at] = more ? gb[at] + ab[e] : ab[e];
     }
 }
 
 // ---------------------------------------------------------------- host
-constexpr int64_t kRowsPerLaunch = 32768;     // a grid's y extent is below 65536
+// Rows of one launch: at most 32768 (a grid's y extent).  Forward also at most 144 MB of x where there is more, so that the second read
+// of a row comes from the last-level cache (256 MB): 3355 rows of 20000 fp32 columns 234 us in one go, 198 in two.  Backward, where
+// the second pass reads and writes as much again, the same made it slower (331 and 416 us): one go.
+int64_t rows_at_once(int64_t rows, int64_t row_bytes) {
+  int64_t parts = (rows * row_bytes + ((int64_t)144 << 20) - 1) / ((int64_t)144 << 20);
+  if (parts < 1) parts = 1;
+  const int64_t n = (rows + parts - 1) / parts;
+  return n < 32768 ? n : 32768;
+}
 
-// columns of a chunk: about 1024 chunks in all, 4096 to 16384 columns each (a multiple of 4096), at most 1024 to a row
-int64_t chunk_len(int64_t rows, int64_t cols) {
-  int64_t len = 16384;
-  while (len > 4096 && rows * ((cols + len - 1) / len) < 1024) len >>= 1;
+struct Plan {
+  int64_t most;             // rows at a time
+  int64_t len, chunks;      // columns of a chunk (a multiple of 4096, 16384 where that makes 1024 chunks), chunks of a row (at most 1024)
+  int64_t groups, span;     // row groups of the last backward pass: enough workgroups for the chip, at least 4 rows each
+};
+Plan plan_of(int64_t rows, int64_t cols, int64_t size, bool backward) {
+  Plan p;
+  p.most = rows_at_once(rows, backward ? 0 : cols * size);
+  p.len = 16384;
+  while (p.len > 4096 && p.most * ((cols + p.len - 1) / p.len) < 1024) p.len >>= 1;
   const int64_t least = ((cols + 1023) / 1024 + 4095) / 4096 * 4096;
-  return len > least ? len : least;
-}
-int64_t chunks_of(int64_t rows, int64_t cols) { return (cols + chunk_len(rows, cols) - 1) / chunk_len(rows, cols); }
-// row groups of the last pass: enough workgroups for the chip, at least 4 rows each
-int64_t groups_of(int64_t rows, int64_t cols) {
+  if (p.len < least) p.len = least;
+  p.chunks = (cols + p.len - 1) / p.len;
   const int64_t wide = (cols + 1023) / 1024;
-  int64_t g = (1024 + wide - 1) / wide;
-  if (g > rows / 4) g = rows / 4;
-  return g < 1 ? 1 : g > 256 ? 256 : g;
+  p.groups = (1024 + wide - 1) / wide;
+  if (p.groups > p.most / 4) p.groups = p.most / 4;
+  p.groups = p.groups < 1 ? 1 : p.groups > 256 ? 256 : p.groups;
+  p.span = (p.most + p.groups - 1) / p.groups;
+  return p;
 }
 
-// lanes of a row: the fewest that hold it with 16 bytes each, up to a wave; then up to 16 elements each; then workgroups
+// lanes of a row.  Up to a wave: the fewest that hold it with 16 bytes each.  Then forward: a wave with up to 16 elements a lane
+// (no barrier), workgroups of 256 and of 1024 lanes.  Backward, which holds five arrays of that length, stays at 8 elements a lane
+// and adds waves instead (800 bf16 columns: 5242 rows in 12 us instead of 25), until 1024 lanes are not enough.
 struct Shape { int G, E, NT; };
-Shape shape_of(int64_t cols, int vec) {
-  for (int G = 4; G <= 64; G *= 2)
+Shape shape_of(int64_t cols, int vec, bool backward) {
+  for (int G = 1; G <= 64; G *= 2)
     if (cols <= (int64_t)G * vec) return {G, vec, 256};
-  for (int E = 8; E <= 16; E *= 2)
-    if (E > vec && cols <= 64 * E) return {64, E, 256};
-  for (int G = 256; G <= 1024; G *= 4)
+  if (!backward)
     for (int E = 8; E <= 16; E *= 2)
-      if (cols <= (int64_t)G * E) return {G, E, G};
+      if (cols <= 64 * E) return {64, E, 256};
+  for (int G = backward ? 64 : 256; G <= 1024; G *= backward ? 2 : 4)
+    for (int E = 8; E <= (backward && G < 1024 ? 8 : 16); E *= 2)
+      if (cols <= (int64_t)G * E) return {G, E, G < 256 ? 256 : G};
   return {0, 0, 0};
 }
-int64_t resident_blocks(int64_t rows, const Shape& s) {
-  const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb;
-  const int64_t most = s.NT == 1024 ? kBlocks / 4 : kBlocks;
-  return need < most ? need : most;
+// Backward every workgroup leaves a partial row of 2 cols numbers: four rounds of rows each where that leaves a workgroup for every
+// CU.  Up to four rounds in all are one workgroup's, which then writes the weight's gradient itself: no second launch.
+int64_t resident_blocks(int64_t rows, const Shape& s, bool backward) {
+  const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb, most = kBlocks * 256 / s.NT;
+  int64_t n = need;
+  if (backward) {
+    if (need <= 4) return 1;
+    if (n > 256) n = need / 4 > 256 ? need / 4 : 256;
+  }
+  return n < most ? n : most;
 }
 
 bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && rows <= (int64_t)1 << 40 && cols <= (int64_t)1 << 31; }
@@ -553,95 +677,127 @@ int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 template <class T, int G, int K, int NT>
 void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, int64_t rows, int64_t cols, float eps, float slope,
                 hipStream_t st) {
-  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}));
+  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, false));
   const float inv = 1.0f / (float)cols;
   if (cols % Vec<T>::N) hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, true>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
   else hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, false>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
 }
 template <class T, int G, int K, int NT>
-void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* part, int64_t rows, int64_t cols, float eps,
-                float slope, hipStream_t st) {
-  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}));
+void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* sw, float* sb, int64_t stride, int64_t rows,
+                int64_t cols, float eps, float slope, hipStream_t st) {
+  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, true));
   const float inv = 1.0f / (float)cols;
-  if (cols % Vec<T>::N) hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, true>), grid, dim3(NT), 0, st, x, w, b, gy, gx, part, rows, (int)cols, inv, eps, slope);
-  else hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, false>), grid, dim3(NT), 0, st, x, w, b, gy, gx, part, rows, (int)cols, inv, eps, slope);
+#define LR_GO(RAGGED, ACT) \
+  hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
+  const bool ragged = cols % Vec<T>::N, act = slope != 1.0f;
+  if (ragged && act) LR_GO(true, true);
+  else if (ragged) LR_GO(true, false);
+  else if (act) LR_GO(false, true);
+  else LR_GO(false, false);
+#undef LR_GO
 }
 
-#define LR_LN_SHAPES(CALL)                                                                          \
-  const Shape s = shape_of(cols, Vec<T>::N);                                                        \
-  constexpr int N = Vec<T>::N;                                                                      \
-  if (s.G == 4) CALL(4, 1, 256);                                                                    \
-  else if (s.G == 8) CALL(8, 1, 256);                                                               \
-  else if (s.G == 16) CALL(16, 1, 256);                                                             \
-  else if (s.G == 32) CALL(32, 1, 256);                                                             \
-  else if (s.G == 64 && s.E == N) CALL(64, 1, 256);                                                 \
-  else if (s.G == 64 && s.E == 8) CALL(64, 8 / N, 256);                                             \
-  else if (s.G == 64) CALL(64, 16 / N, 256);                                                        \
-  else if (s.G == 256 && s.E == 8) CALL(256, 8 / N, 256);                                           \
-  else if (s.G == 256) CALL(256, 16 / N, 256);                                                      \
-  else if (s.E == 8) CALL(1024, 8 / N, 1024);                                                       \
-  else CALL(1024, 16 / N, 1024)
+#define LR_LN_NARROW(CALL)                      \
+  if (s.G == 1) CALL(1, 1, 256);                \
+  else if (s.G == 2) CALL(2, 1, 256);           \
+  else if (s.G == 4) CALL(4, 1, 256);           \
+  else if (s.G == 8) CALL(8, 1, 256);           \
+  else if (s.G == 16) CALL(16, 1, 256);         \
+  else if (s.G == 32) CALL(32, 1, 256);         \
+  else if (s.G == 64 && s.E == N) CALL(64, 1, 256)
 
 template <class T>
 int fwd(const T* x, const float* w, const float* b, T* y, float* stats, float* ws, int64_t rows, int64_t cols, float eps, float slope,
         hipStream_t st) {
   if (cols <= kResident) {
+    constexpr int N = Vec<T>::N;
+    const Shape s = shape_of(cols, N, false);
 #define LR_CALL(G, K, NT) launch_fwd<T, G, K, NT>(x, w, b, y, stats, rows, cols, eps, slope, st)
-    LR_LN_SHAPES(LR_CALL);
+    LR_LN_NARROW(LR_CALL);
+    else if (s.G == 64 && s.E == 8) LR_CALL(64, 8 / N, 256);
+    else if (s.G == 64) LR_CALL(64, 16 / N, 256);
+    else if (s.G == 256 && s.E == 8) LR_CALL(256, 8 / N, 256);
+    else if (s.G == 256) LR_CALL(256, 16 / N, 256);
+    else if (s.E == 8) LR_CALL(1024, 8 / N, 1024);
+    else LR_CALL(1024, 16 / N, 1024);
 #undef LR_CALL
     return lr_launch_status();
   }
-  const int64_t len = chunk_len(rows, cols), chunks = chunks_of(rows, cols);
-  float* sv = stats ? stats : ws + 2 * rows * chunks;
-  for (int64_t r = 0; r < rows; r += kRowsPerLaunch) {
-    const unsigned k = (unsigned)(rows - r < kRowsPerLaunch ? rows - r : kRowsPerLaunch);
+  const Plan p = plan_of(rows, cols, sizeof(T), false);
+  const int64_t len = p.len, chunks = p.chunks, most = p.most;
+  for (int64_t r = 0; r < rows; r += most) {
+    const unsigned k = (unsigned)(rows - r < most ? rows - r : most);
     hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
-    hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, len, eps, sv, r);
-    hipLaunchKernelGGL((chunk_fwd_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, y, sv, cols, len, slope, r);
+    hipLaunchKernelGGL((chunk_fwd_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, y, ws, stats, cols, len, eps, slope, r);
     const int rc = lr_launch_status();
     if (rc != LR_OK) return rc;
   }
   return LR_OK;
 }
 
+int finish(const float* part, int64_t n, int64_t cols, float* gw, float* gb, hipStream_t st) {
+  if (n <= 16) hipLaunchKernelGGL((finish_kernel<1>), dim3((unsigned)((2 * cols + 255) / 256)), dim3(256), 0, st, part, (int)n, cols, gw, gb);
+  else hipLaunchKernelGGL((finish_kernel<32>), dim3((unsigned)((2 * cols + 31) / 32)), dim3(1024), 0, st, part, (int)n, cols, gw, gb);
+  return lr_launch_status();
+}
+
 template <class T>
 int bwd(const T* x, const float* w, const float* b, const T* gy, const float* stats, T* gx, float* gw, float* gb, float* ws,
         int64_t rows, int64_t cols, float eps, float slope, hipStream_t st) {
-  const unsigned fin = (unsigned)((2 * cols + kFinish - 1) / kFinish);
   if (cols <= kResident) {
-    float* part = gw || gb ? ws : nullptr;
-#define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, part, rows, cols, eps, slope, st)
-    LR_LN_SHAPES(LR_CALL);
+    constexpr int N = Vec<T>::N;
+    const Shape s = shape_of(cols, N, true);
+    const int64_t blocks = resident_blocks(rows, s, true);
+    const bool part = blocks > 1 && (gw || gb);
+    float *sw = part ? ws : gw, *sb = part ? ws + cols : gb;
+    const int64_t stride = part ? 2 * cols : 0;
+#define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, sw, sb, stride, rows, cols, eps, slope, st)
+    LR_LN_NARROW(LR_CALL);
+    else if (s.G == 64) LR_CALL(64, 8 / N, 256);
+    else if (s.G == 128) LR_CALL(128, 8 / N, 256);
+    else if (s.G == 256) LR_CALL(256, 8 / N, 256);
+    else if (s.G == 512) LR_CALL(512, 8 / N, 512);
+    else if (s.E == 8) LR_CALL(1024, 8 / N, 1024);
+    else LR_CALL(1024, 16 / N, 1024);
 #undef LR_CALL
     const int rc = lr_launch_status();
     if (rc != LR_OK || !part) return rc;
-    hipLaunchKernelGGL(finish_kernel, dim3(fin), dim3(1024), 0, st, part, (int)resident_blocks(rows, s), cols, gw, gb);
-    return lr_launch_status();
+    return finish(ws, blocks, cols, gw, gb, st);
   }
-  const int64_t len = chunk_len(rows, cols), chunks = chunks_of(rows, cols), groups = groups_of(rows, cols);
+  const Plan p = plan_of(rows, cols, sizeof(T), true);
+  const int64_t len = p.len, chunks = p.chunks, most = p.most, groups = p.groups, span = p.span;
+  const bool inside = span * chunks <= kJoin, direct = groups == 1;
   float* sums = ws + 2 * rows * chunks;
   float* own = sums + up16(2 * rows);
   float* part = own + up16(2 * rows);
-  for (int64_t r = 0; r < rows; r += kRowsPerLaunch) {
-    const unsigned k = (unsigned)(rows - r < kRowsPerLaunch ? rows - r : kRowsPerLaunch);
+  const dim3 grid((unsigned)((cols + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N)), (unsigned)groups);
+  float *sw = direct ? gw : part, *sb = direct ? gb : part + cols;
+  const int64_t stride = direct ? 0 : 2 * cols;
+  const float* sv = stats ? stats : own;
+  const bool act = slope != 1.0f;
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t end = r + most < rows ? r + most : rows;
+    const unsigned k = (unsigned)(end - r);
     if (!stats) {
       hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
       hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, len, eps, own, r);
     }
-    hipLaunchKernelGGL((chunk_sums_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, stats ? stats : own, ws, cols, len, slope, r);
-    hipLaunchKernelGGL(join_sums_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, sums, r);
+    if (act) hipLaunchKernelGGL((chunk_sums_kernel<T, true>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, sv, ws, cols, len, slope, r);
+    else hipLaunchKernelGGL((chunk_sums_kernel<T, false>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, sv, ws, cols, len, slope, r);
+    if (!inside) hipLaunchKernelGGL(join_sums_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, sums, r);
+#define LR_GO(JOIN, ACT)                                                                                                              \
+  hipLaunchKernelGGL((chunk_bwd_kernel<T, JOIN, ACT>), grid, dim3(256), 0, st, x, w, b, gy, sv, inside ? ws : sums, gx, sw, sb, stride, r, \
+                     end, span, (int)chunks, cols, slope, r > 0)
+    if (inside && act) LR_GO(true, true);
+    else if (inside) LR_GO(true, false);
+    else if (act) LR_GO(false, true);
+    else LR_GO(false, false);
+#undef LR_GO
     const int rc = lr_launch_status();
     if (rc != LR_OK) return rc;
   }
-  const int64_t span = (rows + groups - 1) / groups;
-  const int64_t wide = (cols + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N);
-  const bool direct = groups == 1;
-  hipLaunchKernelGGL((chunk_bwd_kernel<T>), dim3((unsigned)wide, (unsigned)groups), dim3(256), 0, st, x, w, b, gy, stats ? stats : own, sums, gx,
-                     direct ? gw : part, direct ? gb : part + cols, direct ? 0 : 2 * cols, rows, span, cols, slope);
-  int rc = lr_launch_status();
-  if (rc != LR_OK || direct || !(gw || gb)) return rc;
-  hipLaunchKernelGGL(finish_kernel, dim3(fin), dim3(1024), 0, st, part, (int)groups, cols, gw, gb);
-  return lr_launch_status();
+  if (direct || !(gw || gb)) return LR_OK;
+  return finish(part, groups, cols, gw, gb, st);
 }
 
 __global__ __launch_bounds__(256) void zero_kernel(float* a, float* b, int64_t n) {
@@ -661,13 +817,12 @@ extern "C" int64_t lr_layer_norm_workspace(int64_t rows, int64_t cols, int backw
   if (cols <= kResident) {
     if (!backward) return 0;
     // the larger of the two types' launches
-    const int64_t a = resident_blocks(rows, shape_of(cols, 4)), b = resident_blocks(rows, shape_of(cols, 8));
-    return 4 * 2 * cols * (a > b ? a : b);
+    const int64_t a = resident_blocks(rows, shape_of(cols, 4, true), true), b = resident_blocks(rows, shape_of(cols, 8, true), true);
+    return a == 1 && b == 1 ? 0 : 4 * 2 * cols * (a > b ? a : b);
   }
-  const int64_t words = 2 * rows * chunks_of(rows, cols);
-  if (!backward) return 4 * (words + 2 * rows);
-  const int64_t groups = groups_of(rows, cols);
-  return 4 * (words + 2 * up16(2 * rows) + (groups > 1 ? 2 * cols * groups : 0));
+  const Plan p = plan_of(rows, cols, 2, backward), q = plan_of(rows, cols, 4, backward);      // the larger of the two types'
+  const int64_t words = 2 * rows * (p.chunks > q.chunks ? p.chunks : q.chunks), groups = p.groups > q.groups ? p.groups : q.groups;
+  return 4 * (words + (backward ? 2 * up16(2 * rows) + (groups > 1 ? 2 * cols * groups : 0) : 0));
 }
 
 extern "C" int lr_layer_norm(const void* x, const float* w, const float* b, void* y, float* stats, void* workspace, int64_t rows,
@@ -691,7 +846,7 @@ extern "C" int lr_layer_norm_bwd(const void* x, const float* w, const float* b, 
     return lr_launch_status();
   }
   if (!gx && !gw && !gb) return LR_OK;
-  if (!x || !gy || !workspace) return LR_ENULL;
+  if (!x || !gy || (!workspace && lr_layer_norm_workspace(rows, cols, 1))) return LR_ENULL;
   float* ws = static_cast<float*>(workspace);
   if (bf16)
     return bwd(static_cast<const uint16_t*>(x), w, b, static_cast<const uint16_t*>(gy), stats, static_cast<uint16_t*>(gx), gw, gb, ws, rows,

@@ -22,7 +22,7 @@ constexpr int kThreads = 256;
 constexpr int kPerThread = 16;                      // elements of a chunk per thread: 4 vectors of 4
 constexpr int kChunk = kThreads * kPerThread;       // a whole number of 32-element scale blocks
 constexpr int kTensors = 64;                        // tensors of one launch: a lane each in the search for a chunk's tensor
-constexpr int kNormBlocks = 512;
+constexpr int kNormBlocks = 1024;
 
 // tensors of one launch, by value in the kernel arguments (at most 4 KB): nothing to upload, nothing that a captured graph could
 // outlive

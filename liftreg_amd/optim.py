@@ -10,7 +10,7 @@ import operator
 import torch
 
 from . import _hip
-from .ops import _stream, _timed
+from .ops import _stream_of, _timed
 
 BLOCK = 32                              # consecutive elements that share a scale in the 8-bit states
 _T = torch.Tensor
@@ -65,25 +65,56 @@ def _scalar(x, dtype, device, name):
     return 1, x.data_ptr()
 
 
+def _gather(columns, kinds, read_only):
+    """(addresses column by column, then the sizes of the first column's tensors: array of 64-bit numbers; n; device index;
+    bfloat16?) of parallel lists of tensors, all checks done (csrc/tensors.cpp).  None: something is not as it must be."""
+    n = len(columns[0])
+    host = array.array("Q", bytes(8 * n * (len(columns) + 1)))
+    info = array.array("i", (0, 0))
+    got = _hip.tensors().lr_gather_tensors(columns, kinds, read_only, host.buffer_info()[0], len(host), info.buffer_info()[0])
+    return (host, n, info[0], info[1]) if got == n else None
+
+
+def _norm_partial(numel, n, device):
+    parts = _hip.lib().lr_grad_norm_partials(numel, n)
+    if parts < 0:
+        _hip.check(int(parts), "lr_grad_norm_partials")
+    return torch.empty((max(1, parts),), dtype=torch.float64, device=device)
+
+
 def grad_norm(grads):
     """The 2-norm of all `grads` together (0-dim float32 tensor): fp64 sums in a fixed order, two launches, no synchronisation.
     grads: float32 or bfloat16 GPU tensors of one type and device, any shapes."""
-    grads, dtype, device, sizes = _first(grads, "grads")
-    with torch.cuda.device(device):
+    grads = list(grads)
+    got = _gather((grads,), b"p", 0) if grads else None
+    if got is None:
+        grads, dtype, device, sizes = _first(grads, "grads")
         addr = _column(grads, "grads", dtype, device, sizes)
-        n = len(sizes)
-        host = array.array("Q", addr + sizes)
-        at = host.buffer_info()[0]
-        lib = _hip.lib()
-        parts = lib.lr_grad_norm_partials(at + 8 * n, n)
-        if parts < 0:
-            _hip.check(int(parts), "lr_grad_norm_partials")
-        partial = torch.empty((max(1, parts),), dtype=torch.float64, device=grads[0].device)
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        with _timed("grad_norm", bytes=sum(sizes) * dtype.itemsize):
-            _hip.check(lib.lr_grad_norm(at, at + 8 * n, n, dtype == torch.bfloat16, partial.data_ptr(), out.data_ptr(), _stream()),
-                       "lr_grad_norm")
+        got = array.array("Q", addr + sizes), len(sizes), device, int(dtype == torch.bfloat16)
+    host, n, device, bf16 = got
+    if torch.cuda.current_device() != device:
+        with torch.cuda.device(device):
+            return grad_norm(grads)
+    at = host.buffer_info()[0]
+    numel = at + 8 * n
+    partial = _norm_partial(numel, n, grads[0].device)
+    out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+    with _timed("grad_norm", bytes=sum(host[n:]) * (2 if bf16 else 4)):
+        _hip.check(_hip.lib().lr_grad_norm(at, numel, n, bf16, partial.data_ptr(), out.data_ptr(), _stream_of(device)), "lr_grad_norm")
     return out
+
+
+def _refuse(params, grads, exp_avgs, exp_avg_sqs, scales):
+    """What is wrong with the lists of an adamw_step, said."""
+    params, dtype, device, sizes = _first(params, "params")
+    eight = bool(scales)
+    written = _column(params, "params", dtype, device, sizes)
+    written += _column(exp_avgs, "exp_avgs", torch.float8_e4m3fn if eight else torch.float32, device, sizes)
+    written += _column(exp_avg_sqs, "exp_avg_sqs", torch.float8_e5m2 if eight else torch.float32, device, sizes)
+    for name, column in zip(("exp_avg_scales", "exp_avg_sq_scales"), scales):
+        written += _column(column, name, torch.float8_e8m0fnu, device, [-(-k // BLOCK) for k in sizes])
+    _column(grads, "grads", dtype, device, sizes)
+    raise ValueError("a parameter or state occurs twice in the call")
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
@@ -105,8 +136,6 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     max_norm: the gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in (they are not written); norm is
     `grad_norm` (0-dim float32 tensor) or, if that is None, the 2-norm of all of `grads`, computed here.  A norm that is not finite
     reaches the parameters.  Returns the norm (0-dim float32 tensor), None without max_norm."""
-    params, dtype, device, sizes = _first(params, "params")
-    grads, exp_avgs, exp_avg_sqs = list(grads), list(exp_avgs), list(exp_avg_sqs)
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
         raise ValueError(f"betas must be in [0, 1), eps and weight_decay not negative; got {betas}, {eps}, {weight_decay}")
@@ -117,53 +146,39 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     if max_norm is not None and not max_norm > 0.0:
         raise ValueError(f"max_norm must be positive, got {max_norm}")
     eight = exp_avg_scales is not None
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    scales = (list(exp_avg_scales), list(exp_avg_sq_scales)) if eight else ()
+    got = _gather((params, grads, exp_avgs, exp_avg_sqs) + scales, b"ppmvss" if eight else b"ppff", 1) if params else None
+    if got is None:
+        _refuse(params, grads, exp_avgs, exp_avg_sqs, scales)
+    host, n, device, bf16 = got
     if torch.cuda.current_device() != device:
         with torch.cuda.device(device):
             return adamw_step(params, grads, exp_avgs, exp_avg_sqs, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
                               max_norm=max_norm, grad_norm=grad_norm, exp_avg_scales=exp_avg_scales,
                               exp_avg_sq_scales=exp_avg_sq_scales, seed=seed)
-    n = len(sizes)
-    p = _column(params, "params", dtype, device, sizes)
-    m = _column(exp_avgs, "exp_avgs", torch.float8_e4m3fn if eight else torch.float32, device, sizes)
-    v = _column(exp_avg_sqs, "exp_avg_sqs", torch.float8_e5m2 if eight else torch.float32, device, sizes)
-    scales = []
-    if eight:
-        blocks = [-(-k // BLOCK) for k in sizes]
-        scales = (_column(list(exp_avg_scales), "exp_avg_scales", torch.float8_e8m0fnu, device, blocks) +
-                  _column(list(exp_avg_sq_scales), "exp_avg_sq_scales", torch.float8_e8m0fnu, device, blocks))
-    g = _column(grads, "grads", dtype, device, sizes)
-    written = [a for a in p + m + v + scales if a]
-    if len(set(written)) != len(written):
-        raise ValueError("a parameter or state occurs twice in the call")
     lr, lr_dev = _scalar(lr, torch.float32, device, "lr")
     step, step_dev = _scalar(step, torch.int64, device, "step")
     if lr < 0.0 or step < 1:
         raise ValueError(f"lr must not be negative and step starts at 1; got {lr}, {step}")
-    host = array.array("Q", p + g + m + v + scales + sizes)
-    at = host.buffer_info()[0]
-    col = [at + 8 * n * k for k in range(7)]
-    numel = col[6] if eight else col[4]
-    lib = _hip.lib()
-    norm, norm_in, partial, out = None, None, None, None
+    at, row = host.buffer_info()[0], 8 * n
+    numel = at + (6 if eight else 4) * row
+    norm = norm_in = partial = out = None
     if max_norm is not None:
         norm = grad_norm
         if norm is None:
-            parts = lib.lr_grad_norm_partials(numel, n)
-            if parts < 0:
-                _hip.check(int(parts), "lr_grad_norm_partials")
-            partial = torch.empty((max(1, parts),), dtype=torch.float64, device=params[0].device)
+            partial = _norm_partial(numel, n, params[0].device)
             norm = torch.empty((), dtype=torch.float32, device=params[0].device)
             out = norm.data_ptr()
         else:
             norm_in = _scalar(norm, torch.float32, device, "grad_norm")[1]
             if norm_in is None:
                 raise TypeError("grad_norm: expected a 0-dim float32 tensor")
-    total = sum(sizes)
-    with _timed("adamw_step", bytes=total * (3 * dtype.itemsize + (4 if eight else 16))):
-        _hip.check(lib.lr_adamw_step(col[0], col[1], col[2], col[3], col[4] if eight else None, col[5] if eight else None, numel, n,
-                                     dtype == torch.bfloat16, lr, b1, b2, eps, weight_decay, step, lr_dev, step_dev, max_norm or 0.0,
-                                     norm_in, None if partial is None else partial.data_ptr(), out, seed & 0xFFFFFFFFFFFFFFFF,
-                                     _stream()), "lr_adamw_step")
+    with _timed("adamw_step", bytes=sum(host[-n:]) * (3 * (2 if bf16 else 4) + (4 if eight else 16))):
+        _hip.check(_hip.lib().lr_adamw_step(at, at + row, at + 2 * row, at + 3 * row, at + 4 * row if eight else None,
+                                            at + 5 * row if eight else None, numel, n, bf16, lr, b1, b2, eps, weight_decay, step, lr_dev,
+                                            step_dev, max_norm or 0.0, norm_in, None if partial is None else partial.data_ptr(), out,
+                                            seed & 0xFFFFFFFFFFFFFFFF, _stream_of(device)), "lr_adamw_step")
     torch.autograd.graph.increment_version(params)     # written behind autograd's back: caches keyed on the version see it
     return norm
 

@@ -53,7 +53,8 @@ def test_c_entries_refuse(hip):
     assert lib.lr_layer_norm(f, None, None, f, None, None, 1, long, 0, 1e-5, 1.0, None) == -2
     assert lib.lr_layer_norm(None, None, None, None, None, None, 0, 4, 0, 1e-5, 1.0, None) == 0
     assert lib.lr_layer_norm_bwd(f, None, None, None, None, f, None, None, f, 1, 4, 0, 1e-5, 1.0, None) == -2
-    assert lib.lr_layer_norm_bwd(f, None, None, f, None, f, None, None, None, 1, 4, 0, 1e-5, 1.0, None) == -2
+    assert lib.lr_layer_norm_workspace(4, 800, 1) == 0 and lib.lr_layer_norm_workspace(4000, 800, 1) > 0
+    assert lib.lr_layer_norm_bwd(f, None, None, f, None, f, None, None, None, 4000, 800, 0, 1e-5, 1.0, None) == -2
     assert lib.lr_layer_norm_bwd(f, None, None, f, None, None, None, None, f, 1, 4, 0, 1e-5, 1.0, None) == 0
 
 
