@@ -157,22 +157,26 @@ def lib():
     return _lib
 
 
-_tensors = None
+_host = None
 
 
-def tensors():
-    """liblr_tensors.so (csrc/tensors.cpp): lr_gather_tensors, the checks and addresses of lists of tensors in one call."""
-    global _tensors
-    if _tensors is None:
-        path = os.path.join(CSRC, "liblr_tensors.so")
-        if not os.path.exists(path):
-            raise LiftRegHipError(f"{path} not found: build it with `make -C liftreg_amd/csrc`")
-        import torch  # noqa: F401  (its libraries resolve the symbols)
-        handle = C.PyDLL(path)
-        fn = handle.lr_gather_tensors
-        fn.restype, fn.argtypes = _i64, [C.py_object, C.c_char_p, _i, _p, _i64, _p]
-        _tensors = handle
-    return _tensors
+def host():
+    """liftreg_amd._host (csrc/host.cpp), bound to the loaded library: checks, allocations and calls of ops.layer_norm and
+    liftreg_amd.optim in C++."""
+    global _host
+    if _host is None:
+        handle = lib()
+        import torch
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise LiftRegHipError(f"liftreg_amd/_host.so cannot be loaded ({e}): build it with `make -C liftreg_amd/csrc`") from e
+        module.bind(LiftRegHipError, torch._C._cuda_getCurrentRawStream,
+                    *(C.cast(getattr(handle, n), C.c_void_p).value for n in (
+                        "lr_strerror", "lr_layer_norm_resident_cols", "lr_layer_norm_workspace", "lr_layer_norm", "lr_layer_norm_bwd",
+                        "lr_grad_norm_partials", "lr_grad_norm", "lr_adamw_step")))
+        _host = module
+    return _host
 
 
 def has_experimental():

@@ -19,10 +19,12 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPerThread = 16;                      // elements of a chunk per thread: 4 vectors of 4
-constexpr int kChunk = kThreads * kPerThread;       // a whole number of 32-element scale blocks
+// A workgroup takes chunks of ROUNDS * 1024 elements (whole 32-element scale blocks): four rounds where there is work for every wave
+// slot of the chip, one where the launch is latency and more workgroups shorten it (0.55 M elements: 6.4 us with four, 4.8 with one).
+constexpr int kRound = kThreads * 4;
 constexpr int kTensors = 64;                        // tensors of one launch: a lane each in the search for a chunk's tensor
-constexpr int kNormBlocks = 1024;
+constexpr int kBlocks = 2048;                       // four waves each: every wave slot of the 256 CUs
+constexpr int kNormBlocks = 1024;                    // of the norm: each leaves a number that every workgroup of the step adds up again
 
 // tensors of one launch, by value in the kernel arguments (at most 4 KB): nothing to upload, nothing that a captured graph could
 // outlive
@@ -146,15 +148,69 @@ __device__ __forceinline__ void store4b(uint8_t* a, int64_t i, int64_t n, uint32
       if (i + k < n) a[i + k] = (uint8_t)(r >> (8 * k));
 }
 
-// the tensor that chunk c belongs to: lane k holds the end of tensor k
-__device__ __forceinline__ int tensor_of(uint32_t end_of_lane, uint32_t c) {
-  return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(end_of_lane <= c)));
+// The table as the lanes of a wave hold it, lane k tensor k: all of it is fetched at once (kernel arguments are a miss of about a
+// microsecond), and a chunk's tensor is a ballot and a few readlanes away.
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int k) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), k) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, k);
 }
-template <class T>
-__device__ __forceinline__ uint32_t lane_end(const T& t) {
-  const int lane = threadIdx.x & 63;
-  return lane < t.count ? t.end[min(lane, T::kMax - 1)] : 0xffffffffu;
-}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int k) { return (uint32_t)__builtin_amdgcn_readlane((int)v, k); }
+template <class P>
+__device__ __forceinline__ P* lane_ptr(uint64_t v, int k) { return reinterpret_cast<P*>(lane_of(v, k)); }
+
+struct Sizes {               // every table's
+  uint64_t n;
+  uint32_t end;
+  template <class T>
+  __device__ __forceinline__ void fetch(const T& t, int i, bool held) {
+    n = (uint64_t)t.n[i];
+    end = held ? t.end[i] : 0xffffffffu;
+  }
+  // the tensor that chunk c belongs to, its size and the chunk's first element
+  __device__ __forceinline__ int find(uint32_t c, int64_t chunk, int64_t& size, int64_t& base) const {
+    const int k = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(end <= c)));
+    size = (int64_t)lane_of(n, k);
+    base = (int64_t)(c - (k ? lane_of(end, k - 1) : 0u)) * chunk;
+    return k;
+  }
+};
+template <class T> struct Held;
+template <> struct Held<TableG> {
+  Sizes z;
+  uint64_t g;
+  __device__ __forceinline__ explicit Held(const TableG& t) {
+    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
+    z.fetch(t, i, lane < t.count);
+    g = (uint64_t)t.g[i];
+  }
+};
+template <> struct Held<Table32> {
+  Sizes z;
+  uint64_t p, g, m, v;
+  __device__ __forceinline__ explicit Held(const Table32& t) {
+    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
+    z.fetch(t, i, lane < t.count);
+    p = (uint64_t)t.p[i];
+    g = (uint64_t)t.g[i];
+    m = (uint64_t)t.m[i];
+    v = (uint64_t)t.v[i];
+  }
+};
+template <> struct Held<Table8> {
+  Sizes z;
+  uint64_t p, g, m, v, ms, vs;
+  uint32_t pos;
+  __device__ __forceinline__ explicit Held(const Table8& t) {
+    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
+    z.fetch(t, i, lane < t.count);
+    p = (uint64_t)t.p[i];
+    g = (uint64_t)t.g[i];
+    m = (uint64_t)t.m[i];
+    v = (uint64_t)t.v[i];
+    ms = (uint64_t)t.ms[i];
+    vs = (uint64_t)t.vs[i];
+    pos = t.pos[i];
+  }
+};
 
 __device__ __forceinline__ double block_sum(double s) {   // the same order in every block: the same bits
   __shared__ double red[kThreads / 64];
@@ -166,19 +222,20 @@ __device__ __forceinline__ double block_sum(double s) {   // the same order in e
 
 // ---------------------------------------------------------------- the gradients' norm
 // fp64 accumulators: 13 M squares of numbers that span decades; the conversion and the fma hide under the read.
-template <class G>
+template <class G, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void sumsq_kernel(TableG t, double* __restrict__ partial) {
-  const uint32_t ends = lane_end(t), chunks = t.end[t.count - 1];
+  const Held<TableG> held(t);
+  const uint32_t chunks = lane_of(held.z.end, t.count - 1);
   double s = 0.0;
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int k = tensor_of(ends, c);
-    const int64_t n = t.n[k], base = (int64_t)(c - (k ? t.end[k - 1] : 0u)) * kChunk;
-    const G* g = static_cast<const G*>(t.g[k]);
-    F32 x[kPerThread / 4];
+    int64_t n, base;
+    const int k = held.z.find(c, ROUNDS * kRound, n, base);
+    const G* g = lane_ptr<const G>(held.g, k);
+    F32 x[ROUNDS];
 #pragma unroll
-    for (int j = 0; j < kPerThread / 4; ++j) x[j] = load4(g, base + (j * kThreads + threadIdx.x) * 4, n);
+    for (int j = 0; j < ROUNDS; ++j) x[j] = load4(g, base + (j * kThreads + threadIdx.x) * 4, n);
 #pragma unroll
-    for (int j = 0; j < kPerThread / 4; ++j)
+    for (int j = 0; j < ROUNDS; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s = fma((double)x[j].x[e], (double)x[j].x[e], s);
   }
@@ -236,31 +293,42 @@ __device__ __forceinline__ uint32_t code_of(float x, float inv, uint32_t r) {
 typedef float f2 __attribute__((ext_vector_type(2)));
 
 template <class T>
-struct State;   // how a step reads and writes the two moments of 4 elements
+struct State;   // how a step reads and writes the two moments of 4 elements; At: where those of a tensor are
 
 template <>
 struct State<Table32> {
+  struct At {
+    float *m, *v;
+    __device__ __forceinline__ At(const Held<Table32>& h, int k) : m(lane_ptr<float>(h.m, k)), v(lane_ptr<float>(h.v, k)) {}
+  };
   F32 m, v;
-  __device__ __forceinline__ void load(const Table32& t, int k, int64_t i, int64_t n) {
-    m = load4(t.m[k], i, n);
-    v = load4(t.v[k], i, n);
+  __device__ __forceinline__ void load(const At& t, int64_t i, int64_t n) {
+    m = load4(t.m, i, n);
+    v = load4(t.v, i, n);
   }
   __device__ __forceinline__ void open() {}
-  __device__ __forceinline__ void store(const Table32& t, int k, int64_t i, int64_t n, uint32_t) {
-    store4(t.m[k], i, n, m);
-    store4(t.v[k], i, n, v);
+  __device__ __forceinline__ void store(const At& t, int64_t i, int64_t n, uint32_t) {
+    store4(t.m, i, n, m);
+    store4(t.v, i, n, v);
   }
 };
 
 template <>
 struct State<Table8> {
+  struct At {
+    uint8_t *m, *v, *ms, *vs;
+    uint32_t pos;
+    __device__ __forceinline__ At(const Held<Table8>& h, int k)
+        : m(lane_ptr<uint8_t>(h.m, k)), v(lane_ptr<uint8_t>(h.v, k)), ms(lane_ptr<uint8_t>(h.ms, k)), vs(lane_ptr<uint8_t>(h.vs, k)),
+          pos(lane_of(h.pos, k)) {}
+  };
   F32 m, v;
   uint32_t mq, vq, ms, vs;
-  __device__ __forceinline__ void load(const Table8& t, int k, int64_t i, int64_t n) {
-    mq = load4b(t.m[k], i, n);
-    vq = load4b(t.v[k], i, n);
-    ms = i < n ? t.ms[k][i >> 5] : 1u;
-    vs = i < n ? t.vs[k][i >> 5] : 1u;
+  __device__ __forceinline__ void load(const At& t, int64_t i, int64_t n) {
+    mq = load4b(t.m, i, n);
+    vq = load4b(t.v, i, n);
+    ms = i < n ? t.ms[i >> 5] : 1u;
+    vs = i < n ? t.vs[i >> 5] : 1u;
   }
   __device__ __forceinline__ void open() {
     const float a = scale_of(ms), b = scale_of(vs);
@@ -270,24 +338,24 @@ struct State<Table8> {
     v.x[0] = v0[0] * b; v.x[1] = v0[1] * b; v.x[2] = v1[0] * b; v.x[3] = v1[1] * b;
   }
   // every lane of the wave comes here (elements past the end are zeros): the scale is a maximum over 8 lanes
-  __device__ __forceinline__ void store(const Table8& t, int k, int64_t i, int64_t n, uint32_t key) {
+  __device__ __forceinline__ void store(const At& t, int64_t i, int64_t n, uint32_t key) {
     ms = block_scale<7>(m);
     vs = block_scale<14>(v);
     const float a = ms == 255u ? 0.f : __uint_as_float((254u - ms) << 23), b = vs == 255u ? 0.f : __uint_as_float((254u - vs) << 23);
     uint32_t cm = 0, cv = 0;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t r = mix((t.pos[k] + (uint32_t)i + e) ^ key);
+      const uint32_t r = mix((t.pos + (uint32_t)i + e) ^ key);
       const float x = ms == 255u ? 0.f : m.x[e], w = vs == 255u ? 0.f : v.x[e];   // a block that is not finite: scale NaN, codes 0
       cm |= (code_of<3, 7>(x, a, r & 0xffffu) | ((__float_as_uint(x) >> 24) & 0x80u)) << (8 * e);
       const uint32_t c = code_of<2, 15>(w, b, r >> 16);
       cv |= (w > 0.f ? max(c, 1u) : c) << (8 * e);
     }
-    store4b(t.m[k], i, n, cm);
-    store4b(t.v[k], i, n, cv);
+    store4b(t.m, i, n, cm);
+    store4b(t.v, i, n, cv);
     if ((threadIdx.x & 7) == 0 && i < n) {
-      t.ms[k][i >> 5] = (uint8_t)ms;
-      t.vs[k][i >> 5] = (uint8_t)vs;
+      t.ms[i >> 5] = (uint8_t)ms;
+      t.vs[i >> 5] = (uint8_t)vs;
     }
   }
 };
@@ -310,9 +378,10 @@ __host__ __device__ inline Rates rates(const Hyper& h, double lr, int64_t step) 
 }
 
 // Bound by memory: 28 bytes an element with 32-bit states and fp32 parameters, 16 with 8-bit ones.
-template <class P, class T>
+template <class P, class T, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
-  const uint32_t ends = lane_end(t), chunks = t.end[t.count - 1];
+  const Held<T> held(t);
+  const uint32_t chunks = lane_of(held.z.end, t.count - 1);
   Rates r = h.r;
   if (h.lr_dev || h.step_dev) r = rates(h, h.lr_dev ? (double)*h.lr_dev : h.lr, h.step_dev ? *h.step_dev : h.step);
   const float b1 = (float)h.b1, b2 = (float)h.b2, c1 = (float)(1.0 - h.b1), c2 = (float)(1.0 - h.b2);
@@ -332,23 +401,27 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
     coef = coef > 1.0f ? 1.0f : coef;     // NaN stays NaN
   }
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int k = tensor_of(ends, c);
-    const int64_t n = t.n[k], base = (int64_t)(c - (k ? t.end[k - 1] : 0u)) * kChunk;
-    P* pp = static_cast<P*>(t.p[k]);
-    const P* gp = static_cast<const P*>(t.g[k]);
+    int64_t n, base;
+    const int k = held.z.find(c, ROUNDS * kRound, n, base);
+    P* pp = lane_ptr<P>(held.p, k);
+    const P* gp = lane_ptr<const P>(held.g, k);
+    const typename State<T>::At at(held, k);
+    // rounds in flight: with 8-bit states one (61 registers, eight waves a SIMD) beats two (89, five): 13.5 M bf16 parameters 35 and 38 us;
+    // 32-bit states 57 us either way, 44.6 M 246 with one and 243 with two
+    constexpr int Q = ROUNDS < 2 || T::kMax < kTensors ? 1 : 2;
 #pragma unroll
-    for (int j = 0; j < kPerThread / 4; j += 2) {
-      F32 p[2], g[2];
-      State<T> s[2];
+    for (int j = 0; j < ROUNDS; j += Q) {
+      F32 p[Q], g[Q];
+      State<T> s[Q];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < Q; ++q) {
         const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
         g[q] = load4(gp, i, n);
-        s[q].load(t, k, i, n);
+        s[q].load(at, i, n);
         p[q] = load4(pp, i, n);
       }
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      for (int q = 0; q < Q; ++q) {
         const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
         s[q].open();
 #pragma unroll
@@ -361,15 +434,13 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
           p[q].x[e] = p[q].x[e] * r.keep - r.size * (m * __builtin_amdgcn_rcpf(den));
         }
         store4(pp, i, n, p[q]);
-        s[q].store(t, k, i, n, r.key);
+        s[q].store(at, i, n, r.key);
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- host
-uint32_t chunks_of(int64_t n) { return (uint32_t)((n + kChunk - 1) / kChunk); }
-
 bool sizes_ok(const int64_t* numel, int n) {
   if (n < 1) return false;
   for (int i = 0; i < n; ++i)
@@ -377,22 +448,25 @@ bool sizes_ok(const int64_t* numel, int n) {
   return true;
 }
 
-// calls f(first, last, chunks) for each run of at most `most` tensors with elements
+// Calls f(first, last, rounds, chunks) for each run of at most `most` tensors with elements; rounds of a chunk (see kRound): four where
+// that leaves at least `blocks` chunks of one round.
 template <class F>
-int for_launches(const int64_t* numel, int n, int most, F f) {
+int for_launches(const int64_t* numel, int n, int most, int64_t blocks, F f) {
   int first = 0;
   while (first < n) {
     int last = first, held = 0;
-    int64_t chunks = 0;
+    int64_t chunks1 = 0, chunks4 = 0;
     while (last < n && held < most) {
-      const int64_t more = chunks_of(numel[last]);
-      if (chunks + more > 0x7fffffff) break;
-      chunks += more;
+      const int64_t one = (numel[last] + kRound - 1) / kRound, four = (numel[last] + 4 * kRound - 1) / (4 * kRound);
+      if (chunks4 + four > 0x7fffffff) break;
+      chunks1 += one;
+      chunks4 += four;
       held += numel[last] > 0;
       ++last;
     }
+    const bool small = chunks1 <= blocks;
     if (held) {
-      const int rc = f(first, last, (uint32_t)chunks);
+      const int rc = f(first, last, small ? 1 : 4, (uint32_t)(small ? chunks1 : chunks4));
       if (rc != LR_OK) return rc;
     }
     first = last;
@@ -400,27 +474,46 @@ int for_launches(const int64_t* numel, int n, int most, F f) {
   return LR_OK;
 }
 
+// t's sizes and chunk ends of tensors [first, last), calling put(slot, tensor) for each that has elements
+template <class T, class F>
+void fill(T& t, const int64_t* numel, int first, int last, int rounds, F put) {
+  int k = 0;
+  uint32_t end = 0;
+  for (int i = first; i < last; ++i) {
+    if (!numel[i]) continue;
+    put(k, i);
+    t.n[k] = numel[i];
+    t.end[k++] = end += (uint32_t)((numel[i] + rounds * kRound - 1) / (rounds * kRound));
+  }
+  t.count = k;
+}
+
 unsigned norm_blocks(uint32_t chunks) { return chunks < (uint32_t)kNormBlocks ? chunks : (unsigned)kNormBlocks; }
 
 int sumsq_launches(const void* const* grads, const int64_t* numel, int n, int bf16, double* partial, hipStream_t st) {
   int used = 0;
-  return for_launches(numel, n, TableG::kMax, [&](int first, int last, uint32_t chunks) {
+  return for_launches(numel, n, TableG::kMax, kNormBlocks, [&](int first, int last, int rounds, uint32_t chunks) {
     TableG t;
-    int k = 0;
-    uint32_t end = 0;
-    for (int i = first; i < last; ++i) {
-      if (!numel[i]) continue;
-      t.g[k] = grads[i];
-      t.n[k] = numel[i];
-      t.end[k++] = end += chunks_of(numel[i]);
-    }
-    t.count = k;
-    const unsigned nb = norm_blocks(chunks);
-    if (bf16) hipLaunchKernelGGL((sumsq_kernel<uint16_t>), dim3(nb), dim3(kThreads), 0, st, t, partial + used);
-    else hipLaunchKernelGGL((sumsq_kernel<float>), dim3(nb), dim3(kThreads), 0, st, t, partial + used);
-    used += (int)nb;
+    fill(t, numel, first, last, rounds, [&](int k, int i) { t.g[k] = grads[i]; });
+    const dim3 nb(norm_blocks(chunks));
+    double* out = partial + used;
+    used += (int)nb.x;
+    if (bf16 && rounds == 1) hipLaunchKernelGGL((sumsq_kernel<uint16_t, 1>), nb, dim3(kThreads), 0, st, t, out);
+    else if (bf16) hipLaunchKernelGGL((sumsq_kernel<uint16_t, 4>), nb, dim3(kThreads), 0, st, t, out);
+    else if (rounds == 1) hipLaunchKernelGGL((sumsq_kernel<float, 1>), nb, dim3(kThreads), 0, st, t, out);
+    else hipLaunchKernelGGL((sumsq_kernel<float, 4>), nb, dim3(kThreads), 0, st, t, out);
     return lr_launch_status();
   });
+}
+
+template <class T>
+int launch_step(const T& t, const Hyper& h, uint32_t chunks, int rounds, int bf16, hipStream_t st) {
+  const dim3 grid(chunks < (uint32_t)kBlocks ? chunks : (uint32_t)kBlocks);
+  if (bf16 && rounds == 1) hipLaunchKernelGGL((adamw_kernel<uint16_t, T, 1>), grid, dim3(kThreads), 0, st, t, h);
+  else if (bf16) hipLaunchKernelGGL((adamw_kernel<uint16_t, T, 4>), grid, dim3(kThreads), 0, st, t, h);
+  else if (rounds == 1) hipLaunchKernelGGL((adamw_kernel<float, T, 1>), grid, dim3(kThreads), 0, st, t, h);
+  else hipLaunchKernelGGL((adamw_kernel<float, T, 4>), grid, dim3(kThreads), 0, st, t, h);
+  return lr_launch_status();
 }
 
 }  // namespace
@@ -429,7 +522,7 @@ extern "C" int64_t lr_grad_norm_partials(const int64_t* numel, int n) {
   if (!numel) return LR_ENULL;
   if (!sizes_ok(numel, n)) return LR_EINVAL;
   int64_t used = 0;
-  for_launches(numel, n, TableG::kMax, [&](int, int, uint32_t chunks) {
+  for_launches(numel, n, TableG::kMax, kNormBlocks, [&](int, int, int, uint32_t chunks) {
     used += norm_blocks(chunks);
     return LR_OK;
   });
@@ -477,48 +570,30 @@ extern "C" int lr_adamw_step(void* const* params, const void* const* grads, void
       return lr_launch_status();
     }
   }
-  // 2048 blocks of four waves: every wave slot of the 256 CUs
-  auto grid = [](uint32_t chunks) { return dim3(chunks < 2048u ? chunks : 2048u); };
   if (!eight)
-    return for_launches(numel, n, Table32::kMax, [&](int first, int last, uint32_t chunks) {
+    return for_launches(numel, n, Table32::kMax, kBlocks, [&](int first, int last, int rounds, uint32_t chunks) {
       Table32 t;
-      int k = 0;
-      uint32_t end = 0;
-      for (int i = first; i < last; ++i) {
-        if (!numel[i]) continue;
+      fill(t, numel, first, last, rounds, [&](int k, int i) {
         t.p[k] = params[i];
         t.g[k] = grads[i];
         t.m[k] = static_cast<float*>(exp_avg[i]);
         t.v[k] = static_cast<float*>(exp_avg_sq[i]);
-        t.n[k] = numel[i];
-        t.end[k++] = end += chunks_of(numel[i]);
-      }
-      t.count = k;
-      if (bf16) hipLaunchKernelGGL((adamw_kernel<uint16_t, Table32>), grid(chunks), dim3(kThreads), 0, st, t, h);
-      else hipLaunchKernelGGL((adamw_kernel<float, Table32>), grid(chunks), dim3(kThreads), 0, st, t, h);
-      return lr_launch_status();
+      });
+      return launch_step(t, h, chunks, rounds, bf16, st);
     });
   uint32_t pos = 0;
-  return for_launches(numel, n, Table8::kMax, [&](int first, int last, uint32_t chunks) {
+  return for_launches(numel, n, Table8::kMax, kBlocks, [&](int first, int last, int rounds, uint32_t chunks) {
     Table8 t;
-    int k = 0;
-    uint32_t end = 0;
-    for (int i = first; i < last; ++i) {
-      if (!numel[i]) continue;
+    fill(t, numel, first, last, rounds, [&](int k, int i) {
       t.p[k] = params[i];
       t.g[k] = grads[i];
       t.m[k] = static_cast<uint8_t*>(exp_avg[i]);
       t.v[k] = static_cast<uint8_t*>(exp_avg_sq[i]);
       t.ms[k] = static_cast<uint8_t*>(exp_avg_scale[i]);
       t.vs[k] = static_cast<uint8_t*>(exp_avg_sq_scale[i]);
-      t.n[k] = numel[i];
       t.pos[k] = pos;
       pos += (uint32_t)((numel[i] + 31) & ~(int64_t)31);
-      t.end[k++] = end += chunks_of(numel[i]);
-    }
-    t.count = k;
-    if (bf16) hipLaunchKernelGGL((adamw_kernel<uint16_t, Table8>), grid(chunks), dim3(kThreads), 0, st, t, h);
-    else hipLaunchKernelGGL((adamw_kernel<float, Table8>), grid(chunks), dim3(kThreads), 0, st, t, h);
-    return lr_launch_status();
+    });
+    return launch_step(t, h, chunks, rounds, bf16, st);
   });
 }

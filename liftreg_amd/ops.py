@@ -52,13 +52,6 @@ def _stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-def _stream_of(device):
-    """`_stream()` of a device index, for ops that tensors of another device than the current one may reach."""
-    if _hip.AUTOSYNC:
-        _hip.sync_switches()
-    return torch._C._cuda_getCurrentRawStream(device)     # torch.cuda.current_stream() builds a Stream object: 2.7 us instead of 0.1
-
-
 def _host_f32(a, shape_tail, name):
     """Small host-side parameter (poses, spacing) as a contiguous float32 numpy array."""
     if isinstance(a, torch.Tensor):
@@ -797,55 +790,15 @@ def linear_lrelu(x, weight, bias, negative_slope=1.0):
 
 
 # ----------------------------------------------------------------------------- layer norm
-def _norm_args(x, weight, bias, eps):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"x: expected a torch.Tensor, got {type(x).__name__}")
-    if x.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"x: expected float32 or bfloat16, got {x.dtype}")
-    shape = x.shape
-    if not shape or shape[-1] < 1:
-        raise ValueError(f"x must have a last axis to normalise, got shape {tuple(shape)}")
-    if not eps >= 0.0:
-        raise ValueError(f"eps must not be negative, got {eps}")
-    x = _dev(x, "x", x.dtype)
-    if weight is not None:
-        weight = _norm_param(weight, "weight", shape[-1], x)
-    if bias is not None:
-        bias = _norm_param(bias, "bias", shape[-1], x)
-    return x, weight, bias, shape[-1], x.get_device()
-
-
-def _norm_param(t, name, cols, x):
-    t = _dev(t, name)
-    if t.dim() != 1 or t.numel() != cols or t.get_device() != x.get_device():
-        raise ValueError(f"{name} must have shape ({cols},) on {x.device}, got {tuple(t.shape)} on {t.device}")
-    return t
-
-
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5, negative_slope=1.0, return_stats=False):
     """LeakyReLU(layer norm of x over its last axis * weight + bias), one pass (negative_slope = 1: no activation).
     x: (..., C) float32 or bfloat16, any number of rows; weight, bias: (C,) float32 or None; y in x's type, statistics in float32.
     return_stats: (y, stats) for ops_bwd.layer_norm_bwd: a (rows, 2) tensor of mean and 1 / sqrt(var + eps), or None for rows of
     at most lr_layer_norm_resident_cols() columns, whose backward pass recomputes them from the row it holds in registers."""
-    x, w, b, C, device = _norm_args(x, weight, bias, eps)
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return layer_norm(x, w, b, eps=eps, negative_slope=negative_slope, return_stats=return_stats)
-    lib = _hip.lib()
-    rows = x.numel() // C
-    y = torch.empty_like(x)
-    stats = ws = None
-    if C > lib.lr_layer_norm_resident_cols():
-        need = lib.lr_layer_norm_workspace(rows, C, 0)
-        if need < 0:
-            _hip.check(int(need), "lr_layer_norm_workspace")
-        ws = torch.empty((max(16, need),), dtype=torch.uint8, device=x.device)
-        if return_stats:
-            stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
-    with _timed("layer_norm", cols=C, bytes=2 * x.numel() * x.element_size()):
-        _hip.check(lib.lr_layer_norm(x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), _ptr(stats), _ptr(ws), rows, C,
-                                     x.dtype == torch.bfloat16, eps, negative_slope, _stream_of(device)), "lr_layer_norm")
-    return (y, stats) if return_stats else y
+    if _timer is None:
+        return _hip.host().layer_norm(x, weight, bias, eps, negative_slope, return_stats)
+    with _timed("layer_norm", bytes=2 * x.numel() * x.element_size()):
+        return _hip.host().layer_norm(x, weight, bias, eps, negative_slope, return_stats)
 
 
 # ----------------------------------------------------------------------------- K5 PCA

@@ -6,8 +6,8 @@ no CPU/PyTorch fallback.
 """
 import torch
 
-from . import _hip
-from .ops import _dev, _norm_args, _ptr, _stream, _stream_of, _timed
+from . import _hip, ops
+from .ops import _dev, _ptr, _stream, _timed
 
 
 def ncc_bwd(x, y, moments, gout, n_total, variant=_hip.NCC_CONFIGURED):
@@ -397,31 +397,10 @@ def layer_norm_bwd(x, weight, bias, gy, *, eps=1e-5, negative_slope=1.0, stats=N
     asked for).  x: the forward's input, gy: gradient of its output, of x's type and shape.  `stats`: what the forward returned
     with return_stats (None: recomputed here, which rows above lr_layer_norm_resident_cols() columns pay for with one more read of x).
     negative_slope = 1 with a gy that has gone through the LeakyReLU's mask already."""
-    x, w, b, C, device = _norm_args(x, weight, bias, eps)
-    gy = _dev(gy, "gy", x.dtype)
-    if gy.shape != x.shape or gy.get_device() != device:
-        raise ValueError(f"gy must have x's shape {tuple(x.shape)} and device, got {tuple(gy.shape)} on {gy.device}")
-    rows = x.numel() // C
-    if stats is not None:
-        stats = _dev(stats, "stats")
-        if tuple(stats.shape) != (rows, 2) or stats.get_device() != device:
-            raise ValueError(f"stats must be a ({rows}, 2) tensor on {x.device}, got {tuple(stats.shape)} on {stats.device}")
-    if device != torch.cuda.current_device():
-        with torch.cuda.device(device):
-            return layer_norm_bwd(x, w, b, gy, eps=eps, negative_slope=negative_slope, stats=stats, need_gx=need_gx, need_gwb=need_gwb)
-    lib = _hip.lib()
-    gx = torch.empty_like(x) if need_gx else None
-    gw = torch.empty_like(w) if need_gwb and w is not None else None
-    gb = torch.empty_like(b) if need_gwb and b is not None else None
-    need = lib.lr_layer_norm_workspace(rows, C, 1)
-    if need < 0:
-        _hip.check(int(need), "lr_layer_norm_workspace")
-    ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
-    with _timed("layer_norm_bwd", cols=C, bytes=(3 if need_gx else 2) * x.numel() * x.element_size()):
-        _hip.check(lib.lr_layer_norm_bwd(x.data_ptr(), _ptr(w), _ptr(b), gy.data_ptr(), _ptr(stats), _ptr(gx), _ptr(gw), _ptr(gb),
-                                         _ptr(ws), rows, C, x.dtype == torch.bfloat16, eps, negative_slope, _stream_of(device)),
-                   "lr_layer_norm_bwd")
-    return gx, gw, gb
+    if ops._timer is None:
+        return _hip.host().layer_norm_bwd(x, weight, bias, gy, eps, negative_slope, stats, need_gx, need_gwb)
+    with _timed("layer_norm_bwd", bytes=(3 if need_gx else 2) * x.numel() * x.element_size()):
+        return _hip.host().layer_norm_bwd(x, weight, bias, gy, eps, negative_slope, stats, need_gx, need_gwb)
 
 
 def disp_reg_bwd(disp, gout):

@@ -4,117 +4,22 @@ in one launch, its states in 32 bits or in block-scaled 8 bits, and the global n
 The reference trains with `torch.optim.Adam(eps=1e-5)` (src/liftreg/networks/RegistrationNet.py:245), which `AdamW` with
 `weight_decay=0` is.  GPU tensors only; launches go to torch's current stream of the tensors' device.
 """
-import array
-import operator
-
 import torch
 
-from . import _hip
-from .ops import _stream_of, _timed
+from . import _hip, ops
 
 BLOCK = 32                              # consecutive elements that share a scale in the 8-bit states
 _T = torch.Tensor
-_dtype = operator.attrgetter("dtype")
-
-
-def _column(tensors, name, dtype, device, sizes):
-    """The addresses of a list of tensors, after its checks."""
-    if len(tensors) != len(sizes):
-        raise ValueError(f"{name}: {len(tensors)} tensors for {len(sizes)} parameters")
-    for t in tensors:
-        if not isinstance(t, _T):
-            raise TypeError(f"{name}: expected torch.Tensors, got {type(t).__name__}")
-    where = set(map(_T.get_device, tensors))
-    if where != {device}:
-        if -1 in where:
-            raise _hip.LiftRegHipError(f"{name}: a tensor is on the CPU; liftreg_amd ops run on the GPU only (no CPU fallback)")
-        raise ValueError(f"{name}: all tensors must be on the parameters' device, cuda:{device}")
-    kinds = set(map(_dtype, tensors))
-    if kinds != {dtype}:
-        raise TypeError(f"{name}: expected {dtype}, got {', '.join(sorted(map(str, kinds)))}")
-    if list(map(_T.numel, tensors)) != sizes:
-        raise ValueError(f"{name}: the tensors' sizes do not match the parameters'")
-    if not all(map(_T.is_contiguous, tensors)):
-        raise ValueError(f"{name}: tensors must be contiguous")
-    return list(map(_T.data_ptr, tensors))
-
-
-def _first(tensors, name):
-    tensors = list(tensors)
-    if not tensors:
-        raise ValueError(f"{name}: no tensors")
-    t = tensors[0]
-    if not isinstance(t, _T):
-        raise TypeError(f"{name}: expected torch.Tensors, got {type(t).__name__}")
-    if not t.is_cuda:
-        raise _hip.LiftRegHipError(f"{name}: tensor is on {t.device}; liftreg_amd ops run on the GPU only (no CPU fallback)")
-    if t.dtype not in (torch.float32, torch.bfloat16):
-        raise TypeError(f"{name}: expected float32 or bfloat16, got {t.dtype}")
-    for u in tensors:
-        if not isinstance(u, _T):
-            raise TypeError(f"{name}: expected torch.Tensors, got {type(u).__name__}")
-    return tensors, t.dtype, t.get_device(), list(map(_T.numel, tensors))
-
-
-def _scalar(x, dtype, device, name):
-    """(value, device address) of a number, or of a one-element tensor that stays on the device."""
-    if not isinstance(x, _T):
-        return x, None
-    if x.dtype != dtype or x.numel() != 1 or x.get_device() != device:
-        raise ValueError(f"{name}: a tensor must be one {dtype} on cuda:{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    return 1, x.data_ptr()
-
-
-def _gather(columns, kinds, read_only):
-    """(addresses column by column, then the sizes of the first column's tensors: array of 64-bit numbers; n; device index;
-    bfloat16?) of parallel lists of tensors, all checks done (csrc/tensors.cpp).  None: something is not as it must be."""
-    n = len(columns[0])
-    host = array.array("Q", bytes(8 * n * (len(columns) + 1)))
-    info = array.array("i", (0, 0))
-    got = _hip.tensors().lr_gather_tensors(columns, kinds, read_only, host.buffer_info()[0], len(host), info.buffer_info()[0])
-    return (host, n, info[0], info[1]) if got == n else None
-
-
-def _norm_partial(numel, n, device):
-    parts = _hip.lib().lr_grad_norm_partials(numel, n)
-    if parts < 0:
-        _hip.check(int(parts), "lr_grad_norm_partials")
-    return torch.empty((max(1, parts),), dtype=torch.float64, device=device)
 
 
 def grad_norm(grads):
     """The 2-norm of all `grads` together (0-dim float32 tensor): fp64 sums in a fixed order, two launches, no synchronisation.
-    grads: float32 or bfloat16 GPU tensors of one type and device, any shapes."""
+    grads: contiguous float32 or bfloat16 GPU tensors of one type and device, any shapes."""
+    if ops._timer is None:
+        return _hip.host().grad_norm(grads)
     grads = list(grads)
-    got = _gather((grads,), b"p", 0) if grads else None
-    if got is None:
-        grads, dtype, device, sizes = _first(grads, "grads")
-        addr = _column(grads, "grads", dtype, device, sizes)
-        got = array.array("Q", addr + sizes), len(sizes), device, int(dtype == torch.bfloat16)
-    host, n, device, bf16 = got
-    if torch.cuda.current_device() != device:
-        with torch.cuda.device(device):
-            return grad_norm(grads)
-    at = host.buffer_info()[0]
-    numel = at + 8 * n
-    partial = _norm_partial(numel, n, grads[0].device)
-    out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-    with _timed("grad_norm", bytes=sum(host[n:]) * (2 if bf16 else 4)):
-        _hip.check(_hip.lib().lr_grad_norm(at, numel, n, bf16, partial.data_ptr(), out.data_ptr(), _stream_of(device)), "lr_grad_norm")
-    return out
-
-
-def _refuse(params, grads, exp_avgs, exp_avg_sqs, scales):
-    """What is wrong with the lists of an adamw_step, said."""
-    params, dtype, device, sizes = _first(params, "params")
-    eight = bool(scales)
-    written = _column(params, "params", dtype, device, sizes)
-    written += _column(exp_avgs, "exp_avgs", torch.float8_e4m3fn if eight else torch.float32, device, sizes)
-    written += _column(exp_avg_sqs, "exp_avg_sqs", torch.float8_e5m2 if eight else torch.float32, device, sizes)
-    for name, column in zip(("exp_avg_scales", "exp_avg_sq_scales"), scales):
-        written += _column(column, name, torch.float8_e8m0fnu, device, [-(-k // BLOCK) for k in sizes])
-    _column(grads, "grads", dtype, device, sizes)
-    raise ValueError("a parameter or state occurs twice in the call")
+    with ops._timed("grad_norm", bytes=sum(g.numel() * g.element_size() for g in grads)):
+        return _hip.host().grad_norm(grads)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=None,
@@ -137,50 +42,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     `grad_norm` (0-dim float32 tensor) or, if that is None, the 2-norm of all of `grads`, computed here.  A norm that is not finite
     reaches the parameters.  Returns the norm (0-dim float32 tensor), None without max_norm."""
     b1, b2 = betas
-    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
-        raise ValueError(f"betas must be in [0, 1), eps and weight_decay not negative; got {betas}, {eps}, {weight_decay}")
-    if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
-        raise ValueError("8-bit states need both exp_avg_scales and exp_avg_sq_scales")
-    if max_norm is None and grad_norm is not None:
-        raise ValueError("grad_norm is for max_norm")
-    if max_norm is not None and not max_norm > 0.0:
-        raise ValueError(f"max_norm must be positive, got {max_norm}")
-    eight = exp_avg_scales is not None
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
-    scales = (list(exp_avg_scales), list(exp_avg_sq_scales)) if eight else ()
-    got = _gather((params, grads, exp_avgs, exp_avg_sqs) + scales, b"ppmvss" if eight else b"ppff", 1) if params else None
-    if got is None:
-        _refuse(params, grads, exp_avgs, exp_avg_sqs, scales)
-    host, n, device, bf16 = got
-    if torch.cuda.current_device() != device:
-        with torch.cuda.device(device):
-            return adamw_step(params, grads, exp_avgs, exp_avg_sqs, step=step, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                              max_norm=max_norm, grad_norm=grad_norm, exp_avg_scales=exp_avg_scales,
-                              exp_avg_sq_scales=exp_avg_sq_scales, seed=seed)
-    lr, lr_dev = _scalar(lr, torch.float32, device, "lr")
-    step, step_dev = _scalar(step, torch.int64, device, "step")
-    if lr < 0.0 or step < 1:
-        raise ValueError(f"lr must not be negative and step starts at 1; got {lr}, {step}")
-    at, row = host.buffer_info()[0], 8 * n
-    numel = at + (6 if eight else 4) * row
-    norm = norm_in = partial = out = None
-    if max_norm is not None:
-        norm = grad_norm
-        if norm is None:
-            partial = _norm_partial(numel, n, params[0].device)
-            norm = torch.empty((), dtype=torch.float32, device=params[0].device)
-            out = norm.data_ptr()
-        else:
-            norm_in = _scalar(norm, torch.float32, device, "grad_norm")[1]
-            if norm_in is None:
-                raise TypeError("grad_norm: expected a 0-dim float32 tensor")
-    with _timed("adamw_step", bytes=sum(host[-n:]) * (3 * (2 if bf16 else 4) + (4 if eight else 16))):
-        _hip.check(_hip.lib().lr_adamw_step(at, at + row, at + 2 * row, at + 3 * row, at + 4 * row if eight else None,
-                                            at + 5 * row if eight else None, numel, n, bf16, lr, b1, b2, eps, weight_decay, step, lr_dev,
-                                            step_dev, max_norm or 0.0, norm_in, None if partial is None else partial.data_ptr(), out,
-                                            seed & 0xFFFFFFFFFFFFFFFF, _stream_of(device)), "lr_adamw_step")
-    torch.autograd.graph.increment_version(params)     # written behind autograd's back: caches keyed on the version see it
-    return norm
+    if ops._timer is not None:
+        params = list(params)
+    args = (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, b1, b2, eps, weight_decay, max_norm, grad_norm, seed)
+    if ops._timer is None:
+        return _hip.host().adamw_step(*args)
+    with ops._timed("adamw_step", bytes=sum(p.numel() * (3 * p.element_size() + (16 if exp_avg_scales is None else 4)) for p in params)):
+        return _hip.host().adamw_step(*args)
 
 
 def state8(p):
