@@ -105,9 +105,24 @@ __device__ __forceinline__ void load_f(const float* a, int64_t c, int64_t C, flo
   }
 }
 
+template <int N>
+__device__ __forceinline__ void store_f(float* a, int64_t c, int64_t C, const float* r) {
+#pragma unroll
+  for (int q = 0; q < N; q += 4) store<true>(a, c + q, C, r + q);
+}
+
 template <int CTRL>
 __device__ __forceinline__ float add_dpp(float x) {
   return x + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+// x + the x of the lane 16 (32) further on, modulo 32 (64): gfx950's row swaps, a tenth of a cross-lane read through LDS
+__device__ __forceinline__ float add_row(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_half(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 // sum over aligned groups of G lanes, in every lane
 template <int G>
@@ -116,8 +131,19 @@ __device__ __forceinline__ float lane_sum(float x) {
   if (G >= 4) x = add_dpp<0x4E>(x);      // pair
   if (G >= 8) x = add_dpp<0x141>(x);     // mirrored half row of 8
   if (G >= 16) x = add_dpp<0x140>(x);    // mirrored row of 16
-  if (G >= 32) x += __shfl_xor(x, 16, 64);
-  if (G >= 64) x += __shfl_xor(x, 32, 64);
+  if (G >= 32) x = add_row(x);
+  if (G >= 64) x = add_half(x);
+  return x;
+}
+// sum over the lanes of a wave that are equal modulo G, in every lane: rotations within a row of 16, then the rows
+template <int G>
+__device__ __forceinline__ float stride_sum(float x) {
+  if (G <= 8) x = add_dpp<0x128>(x);
+  if (G <= 4) x = add_dpp<0x124>(x);
+  if (G <= 2) x = add_dpp<0x122>(x);
+  if (G <= 1) x = add_dpp<0x121>(x);
+  if (G <= 16) x = add_row(x);
+  if (G <= 32) x = add_half(x);
   return x;
 }
 
@@ -221,13 +247,14 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 
 // gx (if set), and this workgroup's sums of g xhat and g at sw, sb (if set) + blockIdx.x * stride.  ACT: there is a LeakyReLU mask
 // (without it b is not needed: 16 of 112 registers at 16 elements a lane).  The next rows are loaded before this round's sums
-// (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.
+// (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.  (A workgroup of 1024
+// with several rows at a time has them all at once.)
 template <class T, int G, int K, int NT, bool RAGGED, bool ACT>
 __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                  const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ sw, float* __restrict__ sb,
                                                  int64_t stride, int64_t rows, int C, float inv, float eps, float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G, E = K * N;
-  constexpr bool AHEAD = E <= 8;
+  constexpr bool AHEAD = E <= 8 && (NT < 1024 || G == NT);
   __shared__ float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
@@ -302,44 +329,41 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
   if (!sw && !sb) return;
   // groups of a wave, then waves
 #pragma unroll
-  for (int i = 0; i < E; ++i)
-    for (int o = G; o < 64; o *= 2) {
-      aw[i] += __shfl_xor(aw[i], o, 64);
-      ab[i] += __shfl_xor(ab[i], o, 64);
-    }
+  for (int i = 0; i < E; ++i) {
+    aw[i] = stride_sum<G>(aw[i]);
+    ab[i] = stride_sum<G>(ab[i]);
+  }
   const int64_t at0 = (int64_t)blockIdx.x * stride;
   if (G == NT) {         // one row at a time: every column has one lane
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int c = (k * G + lane) * N + e;
-        if (c < C) {
-          if (sw) sw[at0 + c] = aw[k * N + e];
-          if (sb) sb[at0 + c] = ab[k * N + e];
-        }
-      }
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * G + lane) * N;
+      if (sw) store_f<N>(sw + at0, c, C, aw + k * N);
+      if (sb) store_f<N>(sb + at0, c, C, ab + k * N);
+    }
     return;
   }
   constexpr int W = G == NT ? 1 : G <= 64 ? NT / 64 : NT / G, L = G == NT ? 1 : G * E;      // sums to add, columns
-  __shared__ float cols[W][2][L];
+  __shared__ float cols[W][L];
   const int set = threadIdx.x / (G <= 64 ? 64 : G), at = threadIdx.x % (G <= 64 ? 64 : G);
-  if (at < G) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        cols[set % W][0][((k * G + at) * N + e) % L] = aw[k * N + e];
-        cols[set % W][1][((k * G + at) * N + e) % L] = ab[k * N + e];
-      }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * C; i += NT) {
-    const int which = i >= C, c = i - which * C;
-    float s = 0.f;
-    for (int q = 0; q < W; ++q) s += cols[q][which][c];
+  for (int which = 0; which < 2; ++which) {
+    const float* part = which ? ab : aw;
     float* out = which ? sb : sw;
-    if (out) out[at0 + c] = s;
+    if (!out) continue;
+    __syncthreads();
+    if (at < G) {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < N; ++e) cols[set % W][((k * G + at) * N + e) % L] = part[k * N + e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < C; c += NT) {
+      float s = 0.f;
+      for (int q = 0; q < W; ++q) s += cols[q][c % L];
+      out[at0 + c] = s;
+    }
   }
 }
 
@@ -643,28 +667,30 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t size, bool backward) {
   return p;
 }
 
-// lanes of a row.  Up to a wave: the fewest that hold it with 16 bytes each.  Then forward: a wave with up to 16 elements a lane
-// (no barrier), workgroups of 256 and of 1024 lanes.  Backward, which holds five arrays of that length, stays at 8 elements a lane
-// and adds waves instead (800 bf16 columns: 5242 rows in 12 us instead of 25), until 1024 lanes are not enough.
+// Lanes of a row: the fewest that hold it with 16 bytes each, up to a wave; then 8 elements a lane (backward holds five arrays of that
+// length, and on few rows fewer loads in a row are shorter: 4099 x 801 forward 10.4 us with 16 elements, 7.5 with 8), until 1024 lanes
+// are not enough.  NT: lanes of a workgroup.  Backward few rows are one workgroup's, which then writes the weight's gradient itself, no
+// partial rows and no second launch: up to four rounds of 256 lanes, or of 1024 two where a row takes more than a wave (8 x 800: 7.7 us
+// in four rounds, 5.6 in one; 128 x 16: 3.2 us with 256 lanes, 3.5 with 1024).
 struct Shape { int G, E, NT; };
-Shape shape_of(int64_t cols, int vec, bool backward) {
-  for (int G = 1; G <= 64; G *= 2)
-    if (cols <= (int64_t)G * vec) return {G, vec, 256};
-  if (!backward)
-    for (int E = 8; E <= 16; E *= 2)
-      if (cols <= 64 * E) return {64, E, 256};
-  for (int G = backward ? 64 : 256; G <= 1024; G *= backward ? 2 : 4)
-    for (int E = 8; E <= (backward && G < 1024 ? 8 : 16); E *= 2)
-      if (cols <= (int64_t)G * E) return {G, E, G < 256 ? 256 : G};
-  return {0, 0, 0};
+Shape shape_of(int64_t rows, int64_t cols, int vec, bool backward) {
+  Shape s = {0, 0, 256};
+  for (int G = 1; G <= 64 && !s.G; G *= 2)
+    if (cols <= (int64_t)G * vec) s.G = G, s.E = vec;
+  for (int G = 64; G <= 1024 && !s.G; G *= 2)
+    for (int E = 8; E <= (G < 1024 ? 8 : 16) && !s.G; E *= 2)
+      if (cols <= (int64_t)G * E) s.G = G, s.E = E;
+  if (s.G > 256) s.NT = s.G;
+  if (backward && s.G > 64 && rows * s.G <= 2 * 1024) s.NT = 1024;
+  return s;
 }
-// Backward every workgroup leaves a partial row of 2 cols numbers: four rounds of rows each where that leaves a workgroup for every
-// CU.  Up to four rounds in all are one workgroup's, which then writes the weight's gradient itself: no second launch.
+bool one_workgroup(int64_t rows, const Shape& s) { return rows * s.G <= (s.G > 64 ? 2 * 1024 : 4 * 256); }
+// Backward every workgroup leaves a partial row of 2 cols numbers: four rounds of rows each where that leaves a workgroup for every CU.
 int64_t resident_blocks(int64_t rows, const Shape& s, bool backward) {
   const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb, most = kBlocks * 256 / s.NT;
   int64_t n = need;
   if (backward) {
-    if (need <= 4) return 1;
+    if (one_workgroup(rows, s)) return 1;
     if (n > 256) n = need / 4 > 256 ? need / 4 : 256;
   }
   return n < most ? n : most;
@@ -690,36 +716,38 @@ void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, 
 #define LR_GO(RAGGED, ACT) \
   hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
   const bool ragged = cols % Vec<T>::N, act = slope != 1.0f;
-  if (ragged && act) LR_GO(true, true);
+  if constexpr (NT == 1024 && G < NT) LR_GO(true, true);      // few rows: latency, which neither changes
+  else if (ragged && act) LR_GO(true, true);
   else if (ragged) LR_GO(true, false);
   else if (act) LR_GO(false, true);
   else LR_GO(false, false);
 #undef LR_GO
 }
 
-#define LR_LN_NARROW(CALL)                      \
-  if (s.G == 1) CALL(1, 1, 256);                \
-  else if (s.G == 2) CALL(2, 1, 256);           \
-  else if (s.G == 4) CALL(4, 1, 256);           \
-  else if (s.G == 8) CALL(8, 1, 256);           \
-  else if (s.G == 16) CALL(16, 1, 256);         \
-  else if (s.G == 32) CALL(32, 1, 256);         \
-  else if (s.G == 64 && s.E == N) CALL(64, 1, 256)
+// CALL(lanes, vectors a lane, workgroup) for shape s
+#define LR_LN_SHAPES(CALL)                                                        \
+  if (s.G == 1) CALL(1, 1, 256);                                                  \
+  else if (s.G == 2) CALL(2, 1, 256);                                             \
+  else if (s.G == 4) CALL(4, 1, 256);                                             \
+  else if (s.G == 8) CALL(8, 1, 256);                                             \
+  else if (s.G == 16) CALL(16, 1, 256);                                           \
+  else if (s.G == 32) CALL(32, 1, 256);                                           \
+  else if (s.G == 64 && s.E == N) CALL(64, 1, 256);                               \
+  else if (s.G == 64) CALL(64, 8 / N, 256);                                       \
+  else if (s.G == 128 && s.NT == 256) CALL(128, 8 / N, 256);                      \
+  else if (s.G == 256 && s.NT == 256) CALL(256, 8 / N, 256);                      \
+  else if (s.G == 512 && s.NT == 512) CALL(512, 8 / N, 512);                      \
+  else if (s.G == 1024 && s.E == 8) CALL(1024, 8 / N, 1024);                      \
+  else if (s.G == 1024) CALL(1024, 16 / N, 1024)
 
 template <class T>
 int fwd(const T* x, const float* w, const float* b, T* y, float* stats, float* ws, int64_t rows, int64_t cols, float eps, float slope,
         hipStream_t st) {
   if (cols <= kResident) {
     constexpr int N = Vec<T>::N;
-    const Shape s = shape_of(cols, N, false);
+    const Shape s = shape_of(rows, cols, N, false);
 #define LR_CALL(G, K, NT) launch_fwd<T, G, K, NT>(x, w, b, y, stats, rows, cols, eps, slope, st)
-    LR_LN_NARROW(LR_CALL);
-    else if (s.G == 64 && s.E == 8) LR_CALL(64, 8 / N, 256);
-    else if (s.G == 64) LR_CALL(64, 16 / N, 256);
-    else if (s.G == 256 && s.E == 8) LR_CALL(256, 8 / N, 256);
-    else if (s.G == 256) LR_CALL(256, 16 / N, 256);
-    else if (s.E == 8) LR_CALL(1024, 8 / N, 1024);
-    else LR_CALL(1024, 16 / N, 1024);
+    LR_LN_SHAPES(LR_CALL);
 #undef LR_CALL
     return lr_launch_status();
   }
@@ -746,19 +774,16 @@ int bwd(const T* x, const float* w, const float* b, const T* gy, const float* st
         int64_t rows, int64_t cols, float eps, float slope, hipStream_t st) {
   if (cols <= kResident) {
     constexpr int N = Vec<T>::N;
-    const Shape s = shape_of(cols, N, true);
+    const Shape s = shape_of(rows, cols, N, true);
     const int64_t blocks = resident_blocks(rows, s, true);
     const bool part = blocks > 1 && (gw || gb);
     float *sw = part ? ws : gw, *sb = part ? ws + cols : gb;
     const int64_t stride = part ? 2 * cols : 0;
 #define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, sw, sb, stride, rows, cols, eps, slope, st)
-    LR_LN_NARROW(LR_CALL);
-    else if (s.G == 64) LR_CALL(64, 8 / N, 256);
-    else if (s.G == 128) LR_CALL(128, 8 / N, 256);
-    else if (s.G == 256) LR_CALL(256, 8 / N, 256);
-    else if (s.G == 512) LR_CALL(512, 8 / N, 512);
-    else if (s.E == 8) LR_CALL(1024, 8 / N, 1024);
-    else LR_CALL(1024, 16 / N, 1024);
+    LR_LN_SHAPES(LR_CALL);
+    else if (s.G == 128) LR_CALL(128, 8 / N, 1024);
+    else if (s.G == 256) LR_CALL(256, 8 / N, 1024);
+    else LR_CALL(512, 8 / N, 1024);
 #undef LR_CALL
     const int rc = lr_launch_status();
     if (rc != LR_OK || !part) return rc;
@@ -817,7 +842,7 @@ extern "C" int64_t lr_layer_norm_workspace(int64_t rows, int64_t cols, int backw
   if (cols <= kResident) {
     if (!backward) return 0;
     // the larger of the two types' launches
-    const int64_t a = resident_blocks(rows, shape_of(cols, 4, true), true), b = resident_blocks(rows, shape_of(cols, 8, true), true);
+    const int64_t a = resident_blocks(rows, shape_of(rows, cols, 4, true), true), b = resident_blocks(rows, shape_of(rows, cols, 8, true), true);
     return a == 1 && b == 1 ? 0 : 4 * 2 * cols * (a > b ? a : b);
   }
   const Plan p = plan_of(rows, cols, 2, backward), q = plan_of(rows, cols, 4, backward);      // the larger of the two types'
