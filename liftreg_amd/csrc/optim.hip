@@ -12,8 +12,8 @@
 // remainder keeps the expected state equal to the unrounded one.  A v that is not zero never rounds to zero (m / eps would follow).
 // The block's largest magnitude is placed in [2^7, 2^8) of e4m3's 448 and in [2^14, 2^15) of e5m2's 57344: rounding up cannot
 // overflow.  The 16 + 16 random bits of an element are a hash of (seed, step, position), so a step can be repeated bit for bit.
-// m and v are formed with the separate roundings of the formula above (no contraction), so that the states do not depend on the
-// compiler; the update itself uses v_sqrt_f32 / v_rcp_f32 (1 ulp each, of a number that is lr times smaller than p).
+// 32-bit states are formed with the separate fp32 roundings of the formula above (no contraction), 8-bit ones in fp64 before their one
+// rounding; the update itself uses v_sqrt_f32 / v_rcp_f32 (1 ulp each, of a number that is lr times smaller than p).
 #include "lr_common.h"
 
 namespace {
@@ -271,23 +271,37 @@ __device__ __forceinline__ float scale_of(uint32_t s) {   // 2^(s - 127); 255 is
   return __uint_as_float(b);
 }
 
-// the exponent byte of the block's scale: its peak lands in [2^top, 2^(top+1))
+__device__ __forceinline__ uint32_t high(double x) { return (uint32_t)(__double_as_longlong(x) >> 32); }
+__device__ __forceinline__ double pow2(int e) { return __longlong_as_double((int64_t)(e + 1023) << 52); }
+
+// the exponent byte of the block's scale: its peak lands in [2^top, 2^(top+1)); 255 where it is beyond fp32 or no number
 template <int TOP>
-__device__ __forceinline__ uint32_t block_scale(const F32& a) {
+__device__ __forceinline__ uint32_t block_scale(const double (&a)[4]) {
   uint32_t u = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) u = max(u, __float_as_uint(a.x[e]) & 0x7fffffffu);
-  const int ex = (int)(max8(u) >> 23);
-  return ex == 255 ? 255u : (uint32_t)max(ex - TOP, 1);
+  for (int e = 0; e < 4; ++e) u = max(u, high(a[e]) & 0x7fffffffu);
+  const int ex = (int)(max8(u) >> 20) - (1023 - 127);
+  return ex > 254 ? 255u : (uint32_t)max(ex - TOP, 1);
 }
 
-// |x| / scale in MAN mantissa bits, exponent bias BIAS, rounded up with the probability of what is cut off
+// |x| / scale in MAN mantissa bits, exponent bias BIAS, rounded up with the probability of what is cut off, for 4 elements.  The random
+// bits end above the low word, which therefore cannot carry.  Below the smallest normal number the steps are even; few waves meet one.
 template <int MAN, int BIAS>
-__device__ __forceinline__ uint32_t code_of(float x, float inv, uint32_t r) {
-  const float y = fabsf(x) * inv;
-  const uint32_t normal = ((__float_as_uint(y) + (r << (23 - MAN - 16))) >> (23 - MAN)) - ((127u - BIAS) << MAN);
-  const uint32_t low = (uint32_t)(y * (float)(1u << (BIAS - 1 + MAN)) + (float)r * 0x1p-16f);
-  return y >= __uint_as_float((128u - BIAS) << 23) ? normal : low;
+__device__ __forceinline__ void codes_of(const double (&x)[4], double inv, const uint32_t (&r)[4], uint32_t (&c)[4]) {
+  constexpr uint32_t NORMAL = (1024u - BIAS) << 20;
+  double y[4];
+  bool low = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    y[e] = fabs(x[e]) * inv;
+    low |= high(y[e]) < NORMAL;
+    c[e] = ((high(y[e]) + (r[e] << (20 - MAN - 16))) >> (20 - MAN)) - ((1023u - BIAS) << MAN);
+  }
+  if (__builtin_expect(__any(low), 0)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (high(y[e]) < NORMAL) c[e] = (uint32_t)(int)fma(y[e], (double)(1u << (BIAS - 1 + MAN)), (double)r[e] * 0x1p-16);
+  }
 }
 
 typedef float f2 __attribute__((ext_vector_type(2)));
@@ -301,15 +315,20 @@ struct State<Table32> {
     float *m, *v;
     __device__ __forceinline__ At(const Held<Table32>& h, int k) : m(lane_ptr<float>(h.m, k)), v(lane_ptr<float>(h.v, k)) {}
   };
-  F32 m, v;
+  typedef float R;           // what the moments are formed in
+  R m[4], v[4];
   __device__ __forceinline__ void load(const At& t, int64_t i, int64_t n) {
-    m = load4(t.m, i, n);
-    v = load4(t.v, i, n);
+    const F32 a = load4(t.m, i, n), b = load4(t.v, i, n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      m[e] = a.x[e];
+      v[e] = b.x[e];
+    }
   }
   __device__ __forceinline__ void open() {}
   __device__ __forceinline__ void store(const At& t, int64_t i, int64_t n, uint32_t) {
-    store4(t.m, i, n, m);
-    store4(t.v, i, n, v);
+    store4(t.m, i, n, {{m[0], m[1], m[2], m[3]}});
+    store4(t.v, i, n, {{v[0], v[1], v[2], v[3]}});
   }
 };
 
@@ -322,7 +341,10 @@ struct State<Table8> {
         : m(lane_ptr<uint8_t>(h.m, k)), v(lane_ptr<uint8_t>(h.v, k)), ms(lane_ptr<uint8_t>(h.ms, k)), vs(lane_ptr<uint8_t>(h.vs, k)),
           pos(lane_of(h.pos, k)) {}
   };
-  F32 m, v;
+  // fp64 runs at fp32's rate here: the stochastic rounding then starts from the moments themselves and not from their fp32 neighbours,
+  // which land on the other side of a code now and then
+  typedef double R;
+  R m[4], v[4];
   uint32_t mq, vq, ms, vs;
   __device__ __forceinline__ void load(const At& t, int64_t i, int64_t n) {
     mq = load4b(t.m, i, n);
@@ -334,25 +356,32 @@ struct State<Table8> {
     const float a = scale_of(ms), b = scale_of(vs);
     const f2 m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mq, true);
     const f2 v0 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vq, false), v1 = __builtin_amdgcn_cvt_pk_f32_bf8((int)vq, true);
-    m.x[0] = m0[0] * a; m.x[1] = m0[1] * a; m.x[2] = m1[0] * a; m.x[3] = m1[1] * a;
-    v.x[0] = v0[0] * b; v.x[1] = v0[1] * b; v.x[2] = v1[0] * b; v.x[3] = v1[1] * b;
+    m[0] = m0[0] * a; m[1] = m0[1] * a; m[2] = m1[0] * a; m[3] = m1[1] * a;
+    v[0] = v0[0] * b; v[1] = v0[1] * b; v[2] = v1[0] * b; v[3] = v1[1] * b;
   }
   // every lane of the wave comes here (elements past the end are zeros): the scale is a maximum over 8 lanes
   __device__ __forceinline__ void store(const At& t, int64_t i, int64_t n, uint32_t key) {
     ms = block_scale<7>(m);
     vs = block_scale<14>(v);
-    const float a = ms == 255u ? 0.f : __uint_as_float((254u - ms) << 23), b = vs == 255u ? 0.f : __uint_as_float((254u - vs) << 23);
-    uint32_t cm = 0, cv = 0;
+    const double a = pow2(127 - (int)ms), b = pow2(127 - (int)vs);
+    uint32_t rm[4], rv[4], cm[4], cv[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t r = mix((t.pos + (uint32_t)i + e) ^ key);
-      const float x = ms == 255u ? 0.f : m.x[e], w = vs == 255u ? 0.f : v.x[e];   // a block that is not finite: scale NaN, codes 0
-      cm |= (code_of<3, 7>(x, a, r & 0xffffu) | ((__float_as_uint(x) >> 24) & 0x80u)) << (8 * e);
-      const uint32_t c = code_of<2, 15>(w, b, r >> 16);
-      cv |= (w > 0.f ? max(c, 1u) : c) << (8 * e);
+      rm[e] = r & 0xffffu;
+      rv[e] = r >> 16;
+      if (ms == 255u) m[e] = 0.0;      // a block that is not finite: scale NaN, codes 0
+      if (vs == 255u) v[e] = 0.0;
     }
-    store4b(t.m, i, n, cm);
-    store4b(t.v, i, n, cv);
+    codes_of<3, 7>(m, a, rm, cm);
+    codes_of<2, 15>(v, b, rv, cv);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cm[e] |= high(m[e]) >> 24 & 0x80u;
+      if (v[e] > 0.0) cv[e] = max(cv[e], 1u);
+    }
+    store4b(t.m, i, n, cm[0] | cm[1] << 8 | cm[2] << 16 | cm[3] << 24);
+    store4b(t.v, i, n, cv[0] | cv[1] << 8 | cv[2] << 16 | cv[3] << 24);
     if ((threadIdx.x & 7) == 0 && i < n) {
       t.ms[i >> 5] = (uint8_t)ms;
       t.vs[i >> 5] = (uint8_t)vs;
@@ -384,21 +413,22 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
   const uint32_t chunks = lane_of(held.z.end, t.count - 1);
   Rates r = h.r;
   if (h.lr_dev || h.step_dev) r = rates(h, h.lr_dev ? (double)*h.lr_dev : h.lr, h.step_dev ? *h.step_dev : h.step);
-  const float b1 = (float)h.b1, b2 = (float)h.b2, c1 = (float)(1.0 - h.b1), c2 = (float)(1.0 - h.b2);
+  typedef typename State<T>::R R;
+  const R b1 = (R)h.b1, b2 = (R)h.b2, c1 = (R)(1.0 - h.b1), c2 = (R)(1.0 - h.b2);
   const float eps = (float)h.eps;
-  float coef = 1.0f;
+  R coef = 1;
   if (h.sumsq || h.norm_in) {
-    float norm;
+    R norm;
     if (h.sumsq) {
       double s = 0.0;
       for (int i = threadIdx.x; i < h.n_sumsq; i += kThreads) s += h.sumsq[i];
-      norm = (float)sqrt(block_sum(s));
-      if (blockIdx.x == 0 && threadIdx.x == 0 && h.norm_out) *h.norm_out = norm;
+      norm = (R)sqrt(block_sum(s));
+      if (blockIdx.x == 0 && threadIdx.x == 0 && h.norm_out) *h.norm_out = (float)norm;
     } else {
       norm = *h.norm_in;
     }
-    coef = h.max_norm / (norm + 1e-6f);
-    coef = coef > 1.0f ? 1.0f : coef;     // NaN stays NaN
+    coef = (R)h.max_norm / (norm + (R)1e-6);
+    coef = coef > (R)1 ? (R)1 : coef;     // NaN stays NaN
   }
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
     int64_t n, base;
@@ -426,12 +456,12 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
         s[q].open();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = g[q].x[e] * coef;
-          const float m = s[q].m.x[e] * b1 + x * c1, v = s[q].v.x[e] * b2 + x * x * c2;
-          s[q].m.x[e] = m;
-          s[q].v.x[e] = v;
-          const float den = fmaf(__builtin_amdgcn_sqrtf(v), r.rbc2, eps);
-          p[q].x[e] = p[q].x[e] * r.keep - r.size * (m * __builtin_amdgcn_rcpf(den));
+          const R x = (R)g[q].x[e] * coef;
+          const R m = s[q].m[e] * b1 + x * c1, v = s[q].v[e] * b2 + x * x * c2;
+          s[q].m[e] = m;
+          s[q].v[e] = v;
+          const float den = fmaf(__builtin_amdgcn_sqrtf((float)v), r.rbc2, eps);
+          p[q].x[e] = p[q].x[e] * r.keep - r.size * ((float)m * __builtin_amdgcn_rcpf(den));
         }
         store4(pp, i, n, p[q]);
         s[q].store(at, i, n, r.key);
