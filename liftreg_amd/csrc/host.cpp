@@ -9,6 +9,8 @@
 #include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
+#include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/liftreg_hip.h"
@@ -227,7 +229,7 @@ struct Columns {
   at::ScalarType type = at::kFloat;
   at::Device device = at::kCPU;
   std::vector<int64_t> numel;
-  std::vector<uint64_t> written;      // addresses that the call writes
+  std::vector<std::pair<uint64_t, uint64_t>> written;      // what the call writes: first byte, end
   std::vector<std::vector<void*>> at;
   std::vector<at::Tensor> keep;       // the first list's tensors
 
@@ -266,14 +268,18 @@ struct Columns {
       if (t.numel() != (blocks ? (numel[i] + 31) / 32 : numel[i])) fail(PyExc_ValueError, std::string(name) + ": the tensors' sizes do not match the parameters'");
       if (!t.is_contiguous()) fail(PyExc_ValueError, std::string(name) + ": tensors must be contiguous");
       column[i] = t.data_ptr();
-      if (writes && t.numel()) written.push_back(reinterpret_cast<uint64_t>(column[i]));
+      if (writes && t.numel()) {
+        const uint64_t from = reinterpret_cast<uint64_t>(column[i]);
+        written.emplace_back(from, from + t.nbytes());
+      }
       if (first) keep.push_back(t);
     }
     at.push_back(std::move(column));
   }
-  void no_twins() {
+  void no_overlap() {
     std::sort(written.begin(), written.end());
-    if (std::adjacent_find(written.begin(), written.end()) != written.end()) fail(PyExc_ValueError, "a parameter or state occurs twice in the call");
+    for (size_t i = 1; i < written.size(); ++i)
+      if (written[i].first < written[i - 1].second) fail(PyExc_ValueError, "parameters or states of the call share memory (is one there twice?)");
   }
   at::Tensor partial() const {
     return empty({std::max<int64_t>(1, count(lr.partials(numel.data(), static_cast<int>(n)), "lr_grad_norm_partials"))}, at::kDouble, device);
@@ -327,7 +333,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c.add(a[5], "exp_avg_sq_scales", at::kFloat8_e8m0fnu, true, true);
     }
     c.add(a[1], "grads", c.type, false, false);
-    c.no_twins();
+    c.no_overlap();
     const float* rate_dev = nullptr;
     const int64_t* step_dev = nullptr;
     double rate = 0.0;

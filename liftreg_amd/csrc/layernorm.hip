@@ -18,6 +18,9 @@
 namespace {
 
 constexpr int kResident = 16384;       // longest row that is held in registers: 1024 lanes of 16 elements
+// arrays from this size on pass the caches by: no line of them would be there when it is read next (the last-level cache holds 256 MB; 1 GB
+// arrays forward + backward 1120 us through the caches, 1089 past them)
+constexpr int64_t kStream = (int64_t)256 << 20;
 constexpr int kBlocks = 2048;          // workgroups of the resident kernels: eight of four waves on each of 256 CUs
 
 template <class T> struct Vec;
@@ -58,7 +61,7 @@ __device__ __forceinline__ void shifted(const uint16_t* row, int64_t c, int64_t 
     r[e + 4] = Vec<uint16_t>::up((uint16_t)(hi >> (16 * e)));
   }
 }
-template <bool RAGGED = true, bool SHIFT = false, class T>
+template <bool RAGGED = true, bool SHIFT = false, bool STREAM = false, class T>
 __device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* r) {
   constexpr int N = Vec<T>::N;
   if constexpr (RAGGED && SHIFT) {
@@ -68,7 +71,8 @@ __device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* 
     }
   }
   if (RAGGED ? c + N <= C : c < C) {
-    const typename Vec<T>::V v = *reinterpret_cast<const typename Vec<T>::V*>(row + c);
+    const typename Vec<T>::V* at = reinterpret_cast<const typename Vec<T>::V*>(row + c);
+    const typename Vec<T>::V v = STREAM ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
     for (int e = 0; e < N; ++e) r[e] = Vec<T>::up(v[e]);
   } else {
@@ -76,14 +80,16 @@ __device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* 
     for (int e = 0; e < N; ++e) r[e] = RAGGED && c + e < C ? Vec<T>::up(row[c + e]) : 0.f;
   }
 }
-template <bool RAGGED = true, class T>
+template <bool RAGGED = true, bool STREAM = false, class T>
 __device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float* r) {
   constexpr int N = Vec<T>::N;
   if (c + N <= C) {
     typename Vec<T>::V v;
 #pragma unroll
     for (int e = 0; e < N; ++e) v[e] = Vec<T>::down(r[e]);
-    *reinterpret_cast<typename Vec<T>::V*>(row + c) = v;
+    typename Vec<T>::V* at = reinterpret_cast<typename Vec<T>::V*>(row + c);
+    if (STREAM) __builtin_nontemporal_store(v, at);
+    else *at = v;
   } else if (RAGGED) {
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -206,7 +212,8 @@ __device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int 
   rstd = __builtin_amdgcn_rsqf(fmaf(gr.sum(q), inv, eps));
 }
 
-template <class T, int G, int K, int NT, bool RAGGED>
+// STREAM: x, gy, y and gx past the caches (kStream).
+template <class T, int G, int K, int NT, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                  T* __restrict__ y, float* __restrict__ stats, int64_t rows, int C, float inv,
                                                  float eps, float slope) {
@@ -226,7 +233,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
     const T* xr = x + r * C;
     float v[K * N];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED>(xr, (k * G + lane) * N, cols, v + k * N);
+    for (int k = 0; k < K; ++k) load<RAGGED, false, STREAM>(xr, (k * G + lane) * N, cols, v + k * N);
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
 #pragma unroll
@@ -236,7 +243,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
         const float z = fmaf((v[k * N + e] - mean) * rstd, wv[k * N + e], bv[k * N + e]);
         v[k * N + e] = z >= 0.f ? z : z * slope;
       }
-      store<RAGGED>(y + r * C, (k * G + lane) * N, cols, v + k * N);
+      store<RAGGED, STREAM>(y + r * C, (k * G + lane) * N, cols, v + k * N);
     }
     if (stats && lane == 0 && r < rows) {
       stats[2 * r] = mean;
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 // (without it b is not needed: 16 of 112 registers at 16 elements a lane).  The next rows are loaded before this round's sums
 // (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.  (A workgroup of 1024
 // with several rows at a time has them all at once.)
-template <class T, int G, int K, int NT, bool RAGGED, bool ACT>
+template <class T, int G, int K, int NT, bool RAGGED, bool ACT, bool STREAM>
 __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                  const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ sw, float* __restrict__ sb,
                                                  int64_t stride, int64_t rows, int C, float inv, float eps, float slope) {
@@ -264,9 +271,9 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
   if (AHEAD) {
     const int cols = r < rows ? C : 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + r * C, (k * G + lane) * N, cols, (AHEAD ? nv : v) + k * N);
+    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + r * C, (k * G + lane) * N, cols, (AHEAD ? nv : v) + k * N);
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + r * C, (k * G + lane) * N, cols, (AHEAD ? ng : g) + k * N);
+    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + r * C, (k * G + lane) * N, cols, (AHEAD ? ng : g) + k * N);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -285,14 +292,14 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
         g[i] = ng[AHEAD ? i : 0];
       }
 #pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? nv : v) + k * N);
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? nv : v) + k * N);
 #pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? ng : g) + k * N);
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? ng : g) + k * N);
     } else {
 #pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(x + r * C, (k * G + lane) * N, cols, v + k * N);
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + r * C, (k * G + lane) * N, cols, v + k * N);
 #pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2>(gy + r * C, (k * G + lane) * N, cols, g + k * N);
+      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + r * C, (k * G + lane) * N, cols, g + k * N);
     }
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
@@ -322,7 +329,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
           const int i = k * N + e;
           v[i] = rstd * (g[i] - fmaf(v[i], s2, s1));
         }
-        store<RAGGED>(gx + r * C, (k * G + lane) * N, cols, v + k * N);
+        store<RAGGED, STREAM>(gx + r * C, (k * G + lane) * N, cols, v + k * N);
       }
     }
   }
@@ -506,7 +513,7 @@ __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x,
       const float z = fmaf((v[e] - mean) * rstd, wv[e], bv[e]);
       v[e] = z >= 0.f ? z : z * slope;
     }
-    store(y + row * C, c, hi, v);
+    store<true, true>(y + row * C, c, hi, v);
   }
 }
 
@@ -624,7 +631,7 @@ __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x,
       ab[e] += gg;
       v[e] = rstd * (gg * wv[e] - fmaf(xh, s2, s1));
     }
-    if (gx) store(gx + r * C, c, C, v);
+    if (gx) store<true, true>(gx + r * C, c, C, v);
   }
 #pragma unroll
   for (int e = 0; e < N; ++e)
@@ -705,22 +712,28 @@ void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, 
                 hipStream_t st) {
   const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, false));
   const float inv = 1.0f / (float)cols;
-  if (cols % Vec<T>::N) hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, true>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
-  else hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, false>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope);
+#define LR_GO(RAGGED, STREAM) \
+  hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, RAGGED, STREAM>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope)
+  if (cols % Vec<T>::N) LR_GO(true, false);
+  else if (rows * cols * (int64_t)sizeof(T) >= kStream) LR_GO(false, true);
+  else LR_GO(false, false);
+#undef LR_GO
 }
 template <class T, int G, int K, int NT>
 void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* sw, float* sb, int64_t stride, int64_t rows,
                 int64_t cols, float eps, float slope, hipStream_t st) {
   const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, true));
   const float inv = 1.0f / (float)cols;
-#define LR_GO(RAGGED, ACT) \
-  hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
-  const bool ragged = cols % Vec<T>::N, act = slope != 1.0f;
-  if constexpr (NT == 1024 && G < NT) LR_GO(true, true);      // few rows: latency, which neither changes
-  else if (ragged && act) LR_GO(true, true);
-  else if (ragged) LR_GO(true, false);
-  else if (act) LR_GO(false, true);
-  else LR_GO(false, false);
+#define LR_GO(RAGGED, ACT, STREAM) \
+  hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT, STREAM>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
+  const bool ragged = cols % Vec<T>::N, act = slope != 1.0f, stream = rows * cols * (int64_t)sizeof(T) >= kStream;
+  if constexpr (NT == 1024 && G < NT) LR_GO(true, true, false);      // few rows: latency, which none of the three changes
+  else if (ragged && act) LR_GO(true, true, false);
+  else if (ragged) LR_GO(true, false, false);
+  else if (act && stream) LR_GO(false, true, true);
+  else if (act) LR_GO(false, true, false);
+  else if (stream) LR_GO(false, false, true);
+  else LR_GO(false, false, false);
 #undef LR_GO
 }
 

@@ -93,11 +93,15 @@ __device__ __forceinline__ uint16_t f_to_bf(float f) {   // nearest even; NaN st
   return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
 }
 
-// 4 elements at i of an array of n (elements past the end read as 0 and are not written)
+// 4 elements at i of an array of n (elements past the end read as 0 and are not written).  ONCE: they are not wanted again before the
+// next step and leave the caches to the gradients, which the norm has read just before (13.5 M parameters with clipping 86 us without,
+// 73 with; 44.6 M without clipping 243 and 225).
+template <bool ONCE>
 __device__ __forceinline__ F32 load4(const float* a, int64_t i, int64_t n) {
   F32 r = {{0.f, 0.f, 0.f, 0.f}};
   if (i + 4 <= n) {
-    const f4 t = *reinterpret_cast<const f4*>(a + i);
+    const f4* at = reinterpret_cast<const f4*>(a + i);
+    const f4 t = ONCE ? __builtin_nontemporal_load(at) : *at;
     r.x[0] = t[0]; r.x[1] = t[1]; r.x[2] = t[2]; r.x[3] = t[3];
   } else {
     for (int k = 0; k < 3; ++k)
@@ -105,10 +109,12 @@ __device__ __forceinline__ F32 load4(const float* a, int64_t i, int64_t n) {
   }
   return r;
 }
+template <bool ONCE>
 __device__ __forceinline__ F32 load4(const uint16_t* a, int64_t i, int64_t n) {
   F32 r = {{0.f, 0.f, 0.f, 0.f}};
   if (i + 4 <= n) {
-    const h4 t = *reinterpret_cast<const h4*>(a + i);
+    const h4* at = reinterpret_cast<const h4*>(a + i);
+    const h4 t = ONCE ? __builtin_nontemporal_load(at) : *at;
     for (int k = 0; k < 4; ++k) r.x[k] = bf_to_f(t[k]);
   } else {
     for (int k = 0; k < 3; ++k)
@@ -119,7 +125,7 @@ __device__ __forceinline__ F32 load4(const uint16_t* a, int64_t i, int64_t n) {
 __device__ __forceinline__ void store4(float* a, int64_t i, int64_t n, const F32& r) {
   if (i + 4 <= n) {
     f4 t = {r.x[0], r.x[1], r.x[2], r.x[3]};
-    *reinterpret_cast<f4*>(a + i) = t;
+    __builtin_nontemporal_store(t, reinterpret_cast<f4*>(a + i));
   } else {
     for (int k = 0; k < 3; ++k)
       if (i + k < n) a[i + k] = r.x[k];
@@ -128,7 +134,7 @@ __device__ __forceinline__ void store4(float* a, int64_t i, int64_t n, const F32
 __device__ __forceinline__ void store4(uint16_t* a, int64_t i, int64_t n, const F32& r) {
   if (i + 4 <= n) {
     h4 t = {f_to_bf(r.x[0]), f_to_bf(r.x[1]), f_to_bf(r.x[2]), f_to_bf(r.x[3])};
-    *reinterpret_cast<h4*>(a + i) = t;
+    __builtin_nontemporal_store(t, reinterpret_cast<h4*>(a + i));
   } else {
     for (int k = 0; k < 3; ++k)
       if (i + k < n) a[i + k] = f_to_bf(r.x[k]);
@@ -233,7 +239,7 @@ __global__ __launch_bounds__(kThreads) void sumsq_kernel(TableG t, double* __res
     const G* g = lane_ptr<const G>(held.g, k);
     F32 x[ROUNDS];
 #pragma unroll
-    for (int j = 0; j < ROUNDS; ++j) x[j] = load4(g, base + (j * kThreads + threadIdx.x) * 4, n);
+    for (int j = 0; j < ROUNDS; ++j) x[j] = load4<false>(g, base + (j * kThreads + threadIdx.x) * 4, n);
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j)
 #pragma unroll
@@ -318,7 +324,7 @@ struct State<Table32> {
   typedef float R;           // what the moments are formed in
   R m[4], v[4];
   __device__ __forceinline__ void load(const At& t, int64_t i, int64_t n) {
-    const F32 a = load4(t.m, i, n), b = load4(t.v, i, n);
+    const F32 a = load4<true>(t.m, i, n), b = load4<true>(t.v, i, n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       m[e] = a.x[e];
@@ -446,9 +452,9 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
 #pragma unroll
       for (int q = 0; q < Q; ++q) {
         const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
-        g[q] = load4(gp, i, n);
+        g[q] = load4<false>(gp, i, n);
         s[q].load(at, i, n);
-        p[q] = load4(pp, i, n);
+        p[q] = load4<true>(pp, i, n);
       }
 #pragma unroll
       for (int q = 0; q < Q; ++q) {

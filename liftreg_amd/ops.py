@@ -797,7 +797,7 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, negative_slope=1.0, retur
     at most lr_layer_norm_resident_cols() columns, whose backward pass recomputes them from the row it holds in registers."""
     if _timer is None:
         return _hip.host().layer_norm(x, weight, bias, eps, negative_slope, return_stats)
-    with _timed("layer_norm", bytes=2 * x.numel() * x.element_size()):
+    with _timed(f"layer_norm_{x.shape[-1]}", bytes=2 * x.numel() * x.element_size()):
         return _hip.host().layer_norm(x, weight, bias, eps, negative_slope, return_stats)
 
 

@@ -399,7 +399,7 @@ def layer_norm_bwd(x, weight, bias, gy, *, eps=1e-5, negative_slope=1.0, stats=N
     negative_slope = 1 with a gy that has gone through the LeakyReLU's mask already."""
     if ops._timer is None:
         return _hip.host().layer_norm_bwd(x, weight, bias, gy, eps, negative_slope, stats, need_gx, need_gwb)
-    with _timed("layer_norm_bwd", bytes=(3 if need_gx else 2) * x.numel() * x.element_size()):
+    with _timed(f"layer_norm_bwd_{x.shape[-1]}", bytes=(3 if need_gx else 2) * x.numel() * x.element_size()):
         return _hip.host().layer_norm_bwd(x, weight, bias, gy, eps, negative_slope, stats, need_gx, need_gwb)
 
 

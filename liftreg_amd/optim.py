@@ -30,14 +30,14 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         p = p (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
 
     params, grads: contiguous float32 or bfloat16 tensors (one type; bfloat16 parameters are rounded to nearest — where lr times
-    the update is below 2^-9 of a parameter it no longer moves: keep those in float32).  No tensor may occur twice.
+    the update is below 2^-9 of a parameter it no longer moves: keep those in float32).  What is written may not overlap.
     exp_avgs, exp_avg_sqs: float32, of the parameters' sizes; or, with exp_avg_scales and exp_avg_sq_scales, block-scaled 8-bit
     states: float8_e4m3fn / float8_e5m2 codes of the parameters' sizes and one float8_e8m0fnu scale for each 32 consecutive
     elements (`state8` makes them, `values8` reads them).  They are rounded stochastically: the random bits are a function of
     (seed, step, position of the element in the call's tensors), so equal calls give equal bits.  A block with an element that is
     not finite becomes NaN as a whole.
     step: 1 for the first step; lr: both numbers, or one-element device tensors (int64, float32) that a captured graph reads
-    at each replay.
+    at each replay (a number is captured as it is).
     max_norm: the gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in (they are not written); norm is
     `grad_norm` (0-dim float32 tensor) or, if that is None, the 2-norm of all of `grads`, computed here.  A norm that is not finite
     reaches the parameters.  Returns the norm (0-dim float32 tensor), None without max_norm."""
@@ -120,6 +120,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
+            raise _hip.LiftRegHipError("a captured step needs capturable=True: the step count would be captured as a number")
         calls, steps = {}, {}
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -132,6 +135,8 @@ class AdamW(torch.optim.Optimizer):
                     raise TypeError(f"gradient is {g.dtype}, its parameter {p.dtype}")
                 s = self.state[p]
                 if not s:
+                    if capturing:
+                        raise _hip.LiftRegHipError("run one step before the capture: the states would start from zero at every replay")
                     s.update(self._new_state(p, steps))
                 # one call for the parameters of a group that have one type, device and step count
                 t = s["step"]

@@ -374,7 +374,7 @@ def test_model_with_norm(dev, size):
     net.train()
     coefs = net.encode(inp["source"], inp["target_proj"], inp["target_poses"])
     want, sd = reference_model(net, inp)
-    assert float((coefs.double() - want).abs().max()) <= 1e-4 * float(want.abs().max())
+    assert float((coefs.double() - want).detach().abs().max()) <= 1e-4 * float(want.detach().abs().max())
     g = torch.randn_like(coefs)
     coefs.backward(g)
     want.backward(g.double())
@@ -401,6 +401,39 @@ def test_model_norm_is_off_by_default_and_refuses_what_is_not_built(dev):
         convBlock(3, 16, layernorm=True, out_layout=ops.LAYOUT_NDHWC_HPS)
     with pytest.raises(ValueError):
         SlabShardedRegistration(make_model(dev, norm="layer"), LocalComm(1))
+
+
+def test_inference_mode_and_shared_weights(dev):
+    from liftreg_amd import ops
+    from liftreg_amd.layers.layers import LayerNorm
+    torch.manual_seed(1)
+    net = LayerNorm(40, negative_slope=0.2).to(dev)
+    x = torch.randn(7, 40, device=dev)
+    want = net(x).detach()
+    with torch.inference_mode():
+        assert torch.equal(net(x), want) and torch.equal(ops.layer_norm(x.clone(), net.weight, net.bias, negative_slope=0.2), want)
+    # one weight used twice, a broadcast input, an expanded gradient: autograd adds them up
+    row = torch.randn(40, device=dev, requires_grad=True)
+    (net(row.expand(5, 40)).sum() + net(x).sum()).backward()
+    g = [p.grad.clone() for p in net.parameters()]
+    gr = row.grad.clone()
+    net.zero_grad(), row.grad.zero_()
+    net(row.expand(5, 40).contiguous()).backward(torch.ones(5, 40, device=dev))
+    net(x).backward(torch.ones(7, 40, device=dev))
+    assert all(torch.equal(a, p.grad) for a, p in zip(g, net.parameters())) and torch.equal(gr, row.grad)
+
+
+def test_graphed_registration_of_the_normalised_model(dev):
+    from liftreg_amd.pipeline import GraphedRegistrar
+    net, inp = make_model(dev, norm="layer").eval(), batch(dev)
+    reg = GraphedRegistrar(net, inp)
+    for k in range(3):
+        inp["source"].uniform_(-1, 1), inp["target_proj"].uniform_(-1, 1)
+        out, _ = reg(inp)
+        with torch.no_grad():
+            want = net(inp)
+        torch.cuda.synchronize()
+        assert torch.equal(out["pca_coefs"], want["pca_coefs"]) and torch.equal(out["warped"], want["warped"]), k
 
 
 @pytest.mark.parametrize("bits", [32, 8])

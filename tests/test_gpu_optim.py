@@ -315,6 +315,11 @@ def test_refusals(dev):
         optim.adamw_step([p[0], p[0]], [g[0], g[0]], [m[0], m[0].clone()], [v[0], v[0].clone()], **ok)
     with pytest.raises(ValueError):
         optim.adamw_step([torch.zeros(8, 8, device=dev).t(), p[1]], g, m, v, **ok)
+    flat = torch.zeros(100, device=dev)
+    with pytest.raises(ValueError):      # overlapping views
+        optim.adamw_step([flat[:64], flat[60:70]], g, m, v, **ok)
+    with pytest.raises(ValueError):      # one element for all of them
+        optim.adamw_step([torch.zeros(1, device=dev).expand(64), p[1]], g, m, v, **ok)
     for more in (dict(step=0), dict(step=1, lr=-1.0), dict(step=1, betas=(1.0, 0.9)), dict(step=1, eps=-1e-8), dict(step=1, weight_decay=-1.0),
                  dict(step=1, max_norm=0.0), dict(step=1, grad_norm=torch.ones((), device=dev)),
                  dict(step=torch.ones((), device=dev)), dict(step=1, lr=torch.ones((), device=dev, dtype=torch.float64)),
@@ -467,3 +472,44 @@ def test_captured_class_step(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(net.parameters(), twin.parameters())), k
     assert int(opt.state[net.a.weight]["step"]) == 5
+
+
+def test_captures_that_could_not_be_replayed_are_refused(dev):
+    from liftreg_amd import _hip, optim
+    for kw, warm in ((dict(), True), (dict(capturable=True), False)):
+        net = Net().to(dev)
+        for p in net.parameters():
+            p.grad = torch.ones_like(p)
+        opt = optim.AdamW(net.parameters(), **kw)
+        if warm:
+            opt.step()
+        before = [p.clone() for p in net.parameters()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(_hip.LiftRegHipError):
+                opt.step()
+            torch.zeros(1, device=dev)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(before, net.parameters()))
+    with pytest.raises(ValueError):
+        optim.AdamW(net.parameters(), lr=torch.tensor(1e-3, device=dev))
+
+
+def test_gradients_in_flat_buckets(dev):
+    """parallel.GradientAllReduce's views (any 4-byte address) as gradients: the bits of separate tensors."""
+    from liftreg_amd import optim
+    from liftreg_amd.parallel import GradientAllReduce
+    torch.manual_seed(6)
+    net = Net().to(dev)
+    twin = copy.deepcopy(net)
+    ddp = GradientAllReduce(net, head_prefix="b.")
+    a, b = optim.AdamW(net.parameters(), max_grad_norm=0.1), optim.AdamW(twin.parameters(), max_grad_norm=0.1)
+    for k in range(3):
+        x = torch.randn(16, 37, device=dev)
+        ddp.zero_grad()
+        net(x).square().mean().backward()
+        ddp.finish()
+        b.zero_grad()
+        twin(x).square().mean().backward()
+        a.step(), b.step()
+        assert all(torch.equal(p, q) for p, q in zip(net.parameters(), twin.parameters())), k
