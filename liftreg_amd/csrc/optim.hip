@@ -39,7 +39,7 @@ struct Table32 {
   int count;
 };
 struct Table8 {
-  static constexpr int kMax = 56;
+  static constexpr int kMax = 61;
   void* p[kMax];
   const void* g[kMax];
   uint8_t* m[kMax];
@@ -52,13 +52,12 @@ struct Table8 {
   int count;
 };
 struct TableG {
-  static constexpr int kMax = kTensors;
+  static constexpr int kMax = 3 * kTensors;      // three tensors a lane
   const void* g[kMax];
   int64_t n[kMax];
   uint32_t end[kMax];
   int count;
 };
-static_assert(sizeof(Table32) <= 3840 && sizeof(Table8) <= 3968 && sizeof(TableG) <= 3840, "kernel arguments are 4 KB");
 
 struct Rates {               // what a step derives from its hyperparameters
   float size, rbc2, keep;
@@ -77,6 +76,9 @@ struct Hyper {
   float max_norm;
   uint64_t seed;
 };
+
+static_assert(sizeof(Table32) + sizeof(Hyper) <= 4096 && sizeof(Table8) + sizeof(Hyper) <= 4096 && sizeof(TableG) + 8 <= 4096,
+              "a launch's arguments are at most 4 KB");
 
 // the alignment of a tensor that is a view into a flat buffer is its element's: gfx950 loads 16 bytes from any dword (or byte)
 // address in one instruction, aligned or not at the same rate where the access is contiguous over the wave
@@ -163,17 +165,19 @@ __device__ __forceinline__ uint32_t lane_of(uint32_t v, int k) { return (uint32_
 template <class P>
 __device__ __forceinline__ P* lane_ptr(uint64_t v, int k) { return reinterpret_cast<P*>(lane_of(v, k)); }
 
-struct Sizes {               // every table's
+struct Sizes {               // every table's, 64 tensors of it
   uint64_t n;
   uint32_t end;
   template <class T>
-  __device__ __forceinline__ void fetch(const T& t, int i, bool held) {
+  __device__ __forceinline__ void fetch(const T& t, int first) {
+    const int lane = threadIdx.x & 63, i = min(first + lane, t.count - 1);
     n = (uint64_t)t.n[i];
-    end = held ? t.end[i] : 0xffffffffu;
+    end = first + lane < t.count ? t.end[i] : 0xffffffffu;
   }
+  __device__ __forceinline__ int before(uint32_t c) const { return (int)__popcll(__ballot(end <= c)); }      // tensors that end there
   // the tensor that chunk c belongs to, its size and the chunk's first element
   __device__ __forceinline__ int find(uint32_t c, int64_t chunk, int64_t& size, int64_t& base) const {
-    const int k = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(end <= c)));
+    const int k = __builtin_amdgcn_readfirstlane(before(c));
     size = (int64_t)lane_of(n, k);
     base = (int64_t)(c - (k ? lane_of(end, k - 1) : 0u)) * chunk;
     return k;
@@ -181,20 +185,37 @@ struct Sizes {               // every table's
 };
 template <class T> struct Held;
 template <> struct Held<TableG> {
-  Sizes z;
-  uint64_t g;
+  Sizes z0, z1, z2;
+  uint64_t g0, g1, g2;
   __device__ __forceinline__ explicit Held(const TableG& t) {
-    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
-    z.fetch(t, i, lane < t.count);
-    g = (uint64_t)t.g[i];
+    const int lane = threadIdx.x & 63, last = t.count - 1;
+    z0.fetch(t, 0);
+    z1.fetch(t, 64);
+    z2.fetch(t, 128);
+    g0 = (uint64_t)t.g[min(lane, last)];
+    g1 = (uint64_t)t.g[min(64 + lane, last)];
+    g2 = (uint64_t)t.g[min(128 + lane, last)];
+  }
+  // readlane from all three, then a scalar choice
+  template <class V>
+  static __device__ __forceinline__ V of(V a, V b, V c, int k) {
+    const V x = lane_of(a, k & 63), y = lane_of(b, k & 63), z = lane_of(c, k & 63);
+    return k < 64 ? x : k < 128 ? y : z;
+  }
+  template <class G>
+  __device__ __forceinline__ const G* find(uint32_t c, int64_t chunk, int64_t& size, int64_t& base) const {
+    const int k = __builtin_amdgcn_readfirstlane(z0.before(c) + z1.before(c) + z2.before(c));
+    size = (int64_t)of(z0.n, z1.n, z2.n, k);
+    base = (int64_t)(c - (k ? of(z0.end, z1.end, z2.end, k - 1) : 0u)) * chunk;
+    return reinterpret_cast<const G*>(of(g0, g1, g2, k));
   }
 };
 template <> struct Held<Table32> {
   Sizes z;
   uint64_t p, g, m, v;
   __device__ __forceinline__ explicit Held(const Table32& t) {
-    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
-    z.fetch(t, i, lane < t.count);
+    const int i = min((int)(threadIdx.x & 63), t.count - 1);
+    z.fetch(t, 0);
     p = (uint64_t)t.p[i];
     g = (uint64_t)t.g[i];
     m = (uint64_t)t.m[i];
@@ -206,8 +227,8 @@ template <> struct Held<Table8> {
   uint64_t p, g, m, v, ms, vs;
   uint32_t pos;
   __device__ __forceinline__ explicit Held(const Table8& t) {
-    const int lane = threadIdx.x & 63, i = min(lane, t.count - 1);
-    z.fetch(t, i, lane < t.count);
+    const int i = min((int)(threadIdx.x & 63), t.count - 1);
+    z.fetch(t, 0);
     p = (uint64_t)t.p[i];
     g = (uint64_t)t.g[i];
     m = (uint64_t)t.m[i];
@@ -231,12 +252,11 @@ __device__ __forceinline__ double block_sum(double s) {   // the same order in e
 template <class G, int ROUNDS>
 __global__ __launch_bounds__(kThreads) void sumsq_kernel(TableG t, double* __restrict__ partial) {
   const Held<TableG> held(t);
-  const uint32_t chunks = lane_of(held.z.end, t.count - 1);
+  const uint32_t chunks = t.end[t.count - 1];
   double s = 0.0;
   for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
     int64_t n, base;
-    const int k = held.z.find(c, ROUNDS * kRound, n, base);
-    const G* g = lane_ptr<const G>(held.g, k);
+    const G* g = held.find<G>(c, ROUNDS * kRound, n, base);
     F32 x[ROUNDS];
 #pragma unroll
     for (int j = 0; j < ROUNDS; ++j) x[j] = load4<false>(g, base + (j * kThreads + threadIdx.x) * 4, n);
