@@ -5,8 +5,8 @@
 //   gw[c] = sum over rows of g xhat,  gb[c] = sum over rows of g
 //
 // Bound by memory: x and y once forward; x, gy and gx once backward.  Two forms, by the length of a row:
-//  * up to kResident columns a row lives in the registers of a group of G lanes (a quarter of a wave for the 16 channels of a voxel,
-//    a wave for the head's 800 features, a workgroup above 1024 columns), 16 bytes a lane and load.  Mean and variance are two
+//  * up to kResident columns a row lives in the registers of a group of G lanes (four for the 16 channels of a voxel, two waves for
+//    the head's 800 features, a workgroup above 1024 columns), 16 bytes a lane and load.  Mean and variance are two
 //    passes over registers.  Backward recomputes them: x is there anyway, and 8 bytes of saved statistics a row would be 1/8 of a
 //    16-channel row forward and again backward.  A lane keeps its columns over all its rows, so the weight's gradient grows in
 //    registers; groups, then waves add theirs, each workgroup leaves one partial row, a second kernel adds those in a fixed order.
