@@ -209,7 +209,8 @@ __device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int 
     }
     q += RAGGED || c < C ? t : 0.f;
   }
-  rstd = __builtin_amdgcn_rsqf(fmaf(gr.sum(q), inv, eps));
+  const float v = fmaf(gr.sum(q), inv, eps);
+  rstd = v < 0x1p-100f ? __builtin_amdgcn_rsqf(v * 0x1p60f) * 0x1p30f : __builtin_amdgcn_rsqf(v);   // v_rsq_f32 takes no subnormals
 }
 
 // STREAM: x, gy, y and gx past the caches (kStream).
@@ -412,7 +413,7 @@ __device__ __forceinline__ Part join(Part a, Part b) {   // Chan: exact up to ro
   r.m2 = a.m2 + b.m2 + d * d * a.n * f;
   return r;
 }
-__device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in thread 0
+__device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in every thread
   __shared__ Part red[4];
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) {
@@ -580,9 +581,8 @@ __global__ __launch_bounds__(256) void join_sums_kernel(const float* __restrict_
 }
 
 // columns of a workgroup, rows [row0 + blockIdx.y * span, + span) below row1: gx, and the columns' sums over these rows (`more`: on top of
-// what is there).  JOIN: the rows' sums of h and
-// h xhat are added up from their chunks here, a wave a row (span rows of `chunks` chunks, at most kJoin in all); else `sums` holds
-// the means.
+// what is there).  JOIN: the rows' sums of h and h xhat are added up from their chunks here, a wave a row (span rows of `chunks` chunks,
+// at most kJoin in all: 2 x 8.4 M columns save a launch of 4.7 us); else `sums` holds the means.
 constexpr int kJoin = 2048;
 template <class T, bool JOIN, bool ACT>
 __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
@@ -703,7 +703,7 @@ int64_t resident_blocks(int64_t rows, const Shape& s, bool backward) {
   return n < most ? n : most;
 }
 
-bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && rows <= (int64_t)1 << 40 && cols <= (int64_t)1 << 31; }
+bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && cols <= (int64_t)1 << 31 && rows <= ((int64_t)1 << 44) / cols; }
 
 int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 

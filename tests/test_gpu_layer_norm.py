@@ -151,6 +151,18 @@ def test_offsets_much_larger_than_the_spread(dev, cols):
     check(dev, x, w, b, gy, 1e-5, 1.0)
 
 
+@pytest.mark.parametrize("cols", [16, 800, 4000, 20_000])
+def test_very_small_and_very_large_values(dev, cols):
+    """Without eps the output does not depend on the input's scale.  At 1e-19 the squares of the differences are subnormal, with down
+    to 12 bits: 2^-11 is allowed; at 1e17 nothing overflows."""
+    from liftreg_amd import ops
+    x, w, b, _ = data(dev, 9, cols, torch.float32, 11)
+    want = definition(x, w, b, 0.0, 1.0)["y"]
+    for scale in (2.0 ** -63, 2.0 ** 56):
+        got = ops.layer_norm(x * scale, w, b, eps=0.0)
+        assert float((got.double() - want).abs().max()) <= 2.0 ** -11 * float(want.abs().max())
+
+
 @pytest.mark.parametrize("cols", [16, 801, 4097, 20_001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_that_start_anywhere(dev, cols, dtype):
