@@ -120,47 +120,34 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-        if capturing and not self.capturable:
-            raise _hip.LiftRegHipError("a captured step needs capturable=True: the step count would be captured as a number")
-        calls, steps = {}, {}
-        for gi, group in enumerate(self.param_groups):
-            for p in group["params"]:
-                g = p.grad
-                if g is None:
-                    continue
-                if g.is_sparse:
-                    raise ValueError("sparse gradients are not supported")
-                if g.dtype != p.dtype:
-                    raise TypeError(f"gradient is {g.dtype}, its parameter {p.dtype}")
-                s = self.state[p]
-                if not s:
-                    if capturing:
-                        raise _hip.LiftRegHipError("run one step before the capture: the states would start from zero at every replay")
-                    s.update(self._new_state(p, steps))
-                # one call for the parameters of a group that have one type, device and step count
-                t = s["step"]
-                key = (gi, p.dtype, p.device, id(t) if isinstance(t, _T) else t)
-                if key not in calls:
-                    calls[key] = ([], [], [])
-                ps, gs, ss = calls[key]
-                ps.append(p)
-                gs.append(g if g.is_contiguous() else g.contiguous())
-                ss.append(s)
         self.grad_norm = None
+        calls, fresh = [], {}
+        for gi, group in enumerate(self.param_groups):
+            ps = [p for p in group["params"] if p.grad is not None]
+            if not ps:
+                continue
+            if ps[0].is_cuda and torch.cuda.is_current_stream_capturing():
+                if not self.capturable:
+                    raise _hip.LiftRegHipError("a captured step needs capturable=True: the step count would be captured as a number")
+                if not all(self.state[p] for p in ps):
+                    raise _hip.LiftRegHipError("run one step before the capture: the states would start from zero at every replay")
+            gs, ss = [p.grad for p in ps], [self.state[p] for p in ps]
+            for p, s in zip(ps, ss):
+                if not s:
+                    s.update(self._new_state(p, fresh))
+            calls += self._calls(gi, ps, [g if g.is_contiguous() else g.contiguous() for g in gs], ss)
         norm = None
         if self.max_grad_norm is not None and len(calls) > 1:
             kinds = {}
-            for (_, dtype, device, _), (_, gs, _) in calls.items():
-                kinds.setdefault((dtype, device), []).extend(gs)
+            for _, ps, gs, _ in calls:
+                kinds.setdefault((ps[0].dtype, ps[0].device), []).extend(gs)
             if len({device for _, device in kinds}) > 1:
                 raise ValueError("max_grad_norm: all parameters must be on one device")
             norms = [grad_norm(gs) for gs in kinds.values()]
             norm = norms[0] if len(norms) == 1 else grad_norm([torch.stack(norms)])
-        counted = set()
-        for (gi, _, _, _), (ps, gs, ss) in calls.items():
-            group = self.param_groups[gi]
-            t = ss[0]["step"]
+        eight, counted = self.state_bits == 8, set()
+        for gi, ps, gs, ss in calls:
+            group, t = self.param_groups[gi], ss[0]["step"]
             if isinstance(t, _T):
                 if id(t) not in counted:      # shared by several calls: counted once
                     counted.add(id(t))
@@ -172,14 +159,26 @@ class AdamW(torch.optim.Optimizer):
             lr = group["lr"]
             if isinstance(lr, _T) and not lr.is_cuda:
                 lr = float(lr)
-            eight = self.state_bits == 8
-            out = adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], step=t, lr=lr, betas=group["betas"],
-                             eps=group["eps"], weight_decay=group["weight_decay"], max_norm=self.max_grad_norm, grad_norm=norm,
-                             exp_avg_scales=[s["exp_avg_scale"] for s in ss] if eight else None,
-                             exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in ss] if eight else None,
-                             seed=self.seed + (gi << 32))      # groups draw different bits
-            self.grad_norm = out
+            self.grad_norm = adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], step=t, lr=lr, betas=group["betas"],
+                                        eps=group["eps"], weight_decay=group["weight_decay"], max_norm=self.max_grad_norm, grad_norm=norm,
+                                        exp_avg_scales=[s["exp_avg_scale"] for s in ss] if eight else None,
+                                        exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in ss] if eight else None,
+                                        seed=self.seed + (gi << 32))      # groups draw different bits
         return loss
+
+    @staticmethod
+    def _calls(gi, ps, gs, ss):
+        """[(group index, params, grads, states)]: one for the parameters of a group that have one type, device and step count."""
+        t = ss[0]["step"]
+        if all(s["step"] is t or (not isinstance(t, _T) and s["step"] == t) for s in ss) and len({p.dtype for p in ps}) == 1 and \
+                len({p.device for p in ps}) == 1:
+            return [(gi, ps, gs, ss)]
+        calls = {}
+        for p, g, s in zip(ps, gs, ss):
+            t = s["step"]
+            c = calls.setdefault((p.dtype, p.device, id(t) if isinstance(t, _T) else t), (gi, [], [], []))
+            c[1].append(p), c[2].append(g), c[3].append(s)
+        return list(calls.values())
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):

@@ -83,7 +83,7 @@ def definition(p, g, m, v, step, lr, eps, wd, max_norm=None, norm=None):
     return p * (1 - lr * wd) - upd, m, v, upd
 
 
-SIZES = [[1], [31, 32, 33], [7, 0, 4096, 4097], [5, 27 * 48, 3, 8191, 70001], [13] * 130]
+SIZES = [[1], [31, 32, 33], [7, 0, 4096, 4097], [5, 27 * 48, 3, 8191, 70001], [13] * 130, [9] * 200]
 
 
 @pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{sum(s)}")
@@ -230,6 +230,8 @@ def test_grad_norm(dev, dtype):
         assert abs(float(got) - want) <= 2 * U32 * want
         assert torch.equal(got, optim.grad_norm(g))
     assert float(optim.grad_norm([torch.empty(0, device=dev)])) == 0.0
+    p = torch.empty(0, device=dev)
+    assert float(optim.adamw_step([p], [p.clone()], [p.clone()], [p.clone()], step=1, max_norm=1.0)) == 0.0
     # squares that leave fp32's range
     big = [torch.full((1000,), 1e30, device=dev), torch.full((1000,), 1e-30, device=dev)]
     assert abs(float(optim.grad_norm(big)) / (1e30 * 1000 ** 0.5) - 1) < 1e-6
