@@ -32,7 +32,7 @@ class LayerNorm(nn.Module):
         if tuple(x.shape[-n:]) != self.normalized_shape:
             raise ValueError(f"the input's trailing axes must be {self.normalized_shape}, got shape {tuple(x.shape)}")
         w, b = (None if t is None else t.reshape(-1) for t in (self.weight, self.bias))
-        y = LayerNormFn.apply(x.reshape(x.shape[:-n] + (-1,)) if n > 1 else x, w, b, self.eps, self.negative_slope, self.premasked_grad)
+        y = LayerNormFn.apply(x.reshape(x.shape[:-n] + (math.prod(self.normalized_shape),)) if n > 1 else x, w, b, self.eps, self.negative_slope, self.premasked_grad)
         return y.view(x.shape) if n > 1 else y
 
 

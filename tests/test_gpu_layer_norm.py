@@ -298,6 +298,7 @@ def test_module_matches_torch(dev):
         assert float((ya - yc).detach().abs().max()) < 200 * U32 * 5 and float((a.grad - c.grad).abs().max()) < 200 * U32 * 5
         for p, q in zip(ref.parameters(), net.parameters()):
             assert p.shape == q.shape and float((p.grad - q.grad).abs().max()) < 200 * U32 * 40
+    assert LayerNorm((4, 6)).to(dev)(torch.empty(0, 4, 6, device=dev)).shape == (0, 4, 6)
     plain = LayerNorm(24, elementwise_affine=False).to(dev)
     assert not list(plain.parameters())
     x = torch.randn(3, 24, device=dev, requires_grad=True)
