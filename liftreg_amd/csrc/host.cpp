@@ -232,15 +232,20 @@ struct Columns {
   std::vector<std::pair<uint64_t, uint64_t>> written;      // what the call writes: first byte, end
   std::vector<std::vector<void*>> at;
   std::vector<at::Tensor> keep;       // the first list's tensors
+  std::vector<PyObject*> lists;       // held until the launches: of a generator's tensors nothing else does, and what they free the call's own
+                                      // workspace would take
+
+  Columns() { lists.reserve(6); }
+  Columns(const Columns&) = delete;
+  ~Columns() {
+    for (PyObject* o : lists) Py_DECREF(o);
+  }
 
   // blocks: one element for each 32 of the first list's tensor
   void add(PyObject* list, const char* name, at::ScalarType want, bool blocks, bool writes) {
     PyObject* fast = PySequence_Fast(list, "expected a list of tensors");
     if (!fast) throw Set();
-    struct Drop {
-      PyObject* o;
-      ~Drop() { Py_DECREF(o); }
-    } drop{fast};
+    lists.push_back(fast);
     const int64_t size = PySequence_Fast_GET_SIZE(fast);
     PyObject** items = PySequence_Fast_ITEMS(fast);
     const bool first = at.empty();
