@@ -30,7 +30,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         p = p (1 - lr weight_decay) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
 
     params, grads: contiguous float32 or bfloat16 tensors (one type; bfloat16 parameters are rounded to nearest — where lr times
-    the update is below 2^-9 of a parameter it no longer moves: keep those in float32).  What is written may not overlap.
+    the update is below 2^-9 of a parameter it no longer moves: keep those in float32).  What is written may not overlap itself
+    (checked) or the gradients.
     exp_avgs, exp_avg_sqs: float32, of the parameters' sizes; or, with exp_avg_scales and exp_avg_sq_scales, block-scaled 8-bit
     states: float8_e4m3fn / float8_e5m2 codes of the parameters' sizes and one float8_e8m0fnu scale for each 32 consecutive
     elements (`state8` makes them, `values8` reads them).  They are rounded stochastically: the random bits are a function of
@@ -40,7 +41,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     at each replay (a number is captured as it is).
     max_norm: the gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in (they are not written); norm is
     `grad_norm` (0-dim float32 tensor) or, if that is None, the 2-norm of all of `grads`, computed here.  A norm that is not finite
-    reaches the parameters.  Returns the norm (0-dim float32 tensor), None without max_norm."""
+    reaches the parameters.  The lists may be any iterables.  Returns the norm (0-dim float32 tensor), None without max_norm."""
     b1, b2 = betas
     if ops._timer is not None:
         params = list(params)
@@ -121,9 +122,10 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         self.grad_norm = None
-        calls, fresh = [], {}
+        calls, fresh, skipped = [], {}, False
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
+            skipped |= len(ps) < len(group["params"])
             if not ps:
                 continue
             if ps[0].is_cuda and torch.cuda.is_current_stream_capturing():
@@ -136,6 +138,8 @@ class AdamW(torch.optim.Optimizer):
                 if not s:
                     s.update(self._new_state(p, fresh))
             calls += self._calls(gi, ps, [g if g.is_contiguous() else g.contiguous() for g in gs], ss)
+        if self.capturable and skipped:
+            self._part_counts(calls)
         norm = None
         if self.max_grad_norm is not None and len(calls) > 1:
             kinds = {}
@@ -154,8 +158,6 @@ class AdamW(torch.optim.Optimizer):
                     t.add_(1)
             else:
                 t += 1
-                for s in ss:
-                    s["step"] = t
             lr = group["lr"]
             if isinstance(lr, _T) and not lr.is_cuda:
                 lr = float(lr)
@@ -164,7 +166,25 @@ class AdamW(torch.optim.Optimizer):
                                         exp_avg_scales=[s["exp_avg_scale"] for s in ss] if eight else None,
                                         exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in ss] if eight else None,
                                         seed=self.seed + (gi << 32))      # groups draw different bits
+            if not isinstance(t, _T):
+                for s in ss:
+                    s["step"] = t
         return loss
+
+    def _part_counts(self, calls):
+        """Parameters that step now leave the device counts that they share with parameters that do not."""
+        now = {id(s) for *_, ss in calls for s in ss}
+        left = {id(s["step"]) for s in self.state.values() if s and id(s) not in now}
+        own = {}
+        for *_, ss in calls:
+            t = ss[0]["step"]
+            if id(t) in left:
+                if torch.cuda.is_current_stream_capturing():
+                    raise _hip.LiftRegHipError("run one step with the same parameters' gradients before the capture: their step count is shared "
+                                               "with parameters that have none")
+                own.setdefault(id(t), t.clone())
+                for s in ss:
+                    s["step"] = own[id(t)]
 
     @staticmethod
     def _calls(gi, ps, gs, ss):
@@ -185,23 +205,25 @@ class AdamW(torch.optim.Optimizer):
         for group in state_dict["param_groups"]:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("amsgrad and maximize are not built")
+            if group.get("weight_decay") and group.get("decoupled_weight_decay") is False:
+                raise ValueError("the checkpoint's weight_decay is an L2 term of the gradient (torch.optim.Adam), which is not built")
         want = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
         for s in state_dict["state"].values():
             if set(s) - {"step"} != want:
                 raise ValueError(f"the checkpoint's states {sorted(s)} are not those of state_bits={self.state_bits}")
-        super().load_state_dict(state_dict)
-        # the base class casts every state to its parameter's type: take the checkpoint's own values again
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ours = [p for g in self.param_groups for p in g["params"]]
+        held = [(p, state_dict["state"][i]) for i, p in zip(ids, ours) if i in state_dict["state"]]
         like = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}[self.state_bits]
-        shared = {}
-        for i, p in zip(ids, ours):
-            if i not in state_dict["state"]:
-                continue
-            src, t = state_dict["state"][i], int(state_dict["state"][i]["step"])
+        for p, src in held:
             for k, dtype in zip(("exp_avg", "exp_avg_sq"), like):
                 if tuple(src[k].shape) != tuple(p.shape) or src[k].dtype != dtype:
                     raise ValueError(f"the checkpoint's {k} is {src[k].dtype} {tuple(src[k].shape)}, needed: {dtype} {tuple(p.shape)}")
+        super().load_state_dict(state_dict)
+        # the base class casts every state to its parameter's type: take the checkpoint's own values again
+        shared = {}
+        for p, src in held:
+            t = int(src["step"])
             if self.capturable:
                 if (p.device, t) not in shared:
                     shared[p.device, t] = torch.tensor(t, dtype=torch.int64, device=p.device)

@@ -292,6 +292,19 @@ def test_streams(dev):
     assert torch.equal(a[0], p[0]) and torch.equal(a[1], m[0]) and torch.equal(a[2], v[0])
 
 
+def test_lists_from_generators(dev):
+    """What a generator yields lives until the launches: the workspace of the norm does not take its memory."""
+    from liftreg_amd import optim
+    sizes = [100] * 100
+    p, g = tensors(dev, sizes, torch.float32, 14)
+    m, v = states32(dev, sizes, 15)
+    a = [[t.clone() for t in ts] for ts in (p, m, v)]
+    want = optim.adamw_step(a[0], [t * 3 for t in g], a[1], a[2], step=1, max_norm=1e-3)
+    got = optim.adamw_step(iter(p), (t * 3 for t in g), iter(m), tuple(v), step=1, max_norm=1e-3)
+    assert torch.equal(got, want) and torch.equal(optim.grad_norm(t * 3 for t in g), want)
+    assert all(torch.equal(x, y) for x, y in zip(a[0] + a[1] + a[2], p + m + v))
+
+
 def test_refusals(dev):
     from liftreg_amd import _hip, optim
     p, g = tensors(dev, [64, 10], torch.float32, 12)
@@ -440,6 +453,49 @@ def test_class_steps_only_what_has_a_gradient(dev):
     before = [p.clone() for p in net.parameters()]
     opt.step()
     assert opt.grad_norm is None and all(torch.equal(a, b) for a, b in zip(before, net.parameters()))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_device_counts_of_parameters_without_gradients(dev, bits):
+    """Parameters that share a count on the device keep their own when only some of them have gradients."""
+    from liftreg_amd import _hip, optim
+    torch.manual_seed(9)
+    net = Net().to(dev)
+    twin = copy.deepcopy(net)
+    opts = [optim.AdamW(n.parameters(), lr=1e-2, max_grad_norm=0.5, state_bits=bits, capturable=c) for n, c in ((net, True), (twin, False))]
+    for k, absent in enumerate(((), ("a.bias",), (), ("a.weight", "a.bias"), ("a.bias",), ())):
+        g = torch.Generator(device="cuda").manual_seed(k)
+        for (name, p), q in zip(net.named_parameters(), twin.parameters()):
+            p.grad = None if name in absent else torch.randn(p.shape, device=dev, generator=g)
+            q.grad = p.grad
+        for o in opts:
+            o.step()
+        for (name, p), q in zip(net.named_parameters(), twin.parameters()):
+            assert torch.equal(p, q), (k, name)
+            assert int(opts[0].state[p]["step"]) == opts[1].state[q]["step"]
+    # within a capture a shared count cannot be parted
+    net2 = Net().to(dev)
+    opt = optim.AdamW(net2.parameters(), capturable=True, state_bits=bits)
+    for p in net2.parameters():
+        p.grad = torch.ones_like(p)
+    opt.step()
+    net2.b.bias.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(_hip.LiftRegHipError):
+            opt.step()
+        torch.zeros(1, device=dev)
+
+
+def test_a_failed_step_is_not_counted(dev):
+    from liftreg_amd import optim
+    net = Net().to(dev)
+    opt = optim.AdamW(net.parameters())
+    train(net, opt, 1)
+    opt.param_groups[0]["eps"] = -1.0
+    with pytest.raises(ValueError):
+        train(net, opt, 1)
+    assert all(s["step"] == 1 for s in opt.state.values())
 
 
 def test_captured_class_step(dev):

@@ -101,6 +101,15 @@ def test_load_state_dict_checks_the_states():
         AdamW(p, state_bits=8).load_state_dict(ref.state_dict())
     with pytest.raises(ValueError):
         AdamW(p).load_state_dict(torch.optim.AdamW(p, amsgrad=True).state_dict())
+    coupled = torch.optim.Adam(p, weight_decay=0.1)
+    with pytest.raises(ValueError):
+        AdamW(p).load_state_dict(coupled.state_dict())
+    AdamW(p).load_state_dict(torch.optim.Adam(p).state_dict())
+    other = [torch.nn.Parameter(torch.ones(41))]
+    fresh = AdamW(other, lr=0.25)
+    with pytest.raises(ValueError):
+        fresh.load_state_dict(ref.state_dict())
+    assert fresh.param_groups[0]["lr"] == 0.25 and not fresh.state
     eight = AdamW(p, state_bits=8)
     m, ms, v, vs = state8(p[0])
     eight.state[p[0]] = {"step": 3, "exp_avg": m, "exp_avg_scale": ms, "exp_avg_sq": v, "exp_avg_sq_scale": vs}
