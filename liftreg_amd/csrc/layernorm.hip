@@ -307,8 +307,9 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
     if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {     // past the end g = 0: nothing is added
-      const float xh = (v[i] - mean) * rstd;
+    for (int i = 0; i < E; ++i) {     // past the end g and xhat are 0 (mean rstd may be beyond fp32): nothing is added
+      const int c = (i / N * G + lane) * N + (RAGGED ? i % N : 0);
+      const float xh = (v[i] - mean) * (c < C ? rstd : 0.f);
       float gg = g[i];
       if (ACT) gg = fmaf(xh, wv[i], bv[ACT ? i : 0]) >= 0.f ? gg : gg * slope;
       aw[i] = fmaf(gg, xh, aw[i]);

@@ -163,6 +163,22 @@ def test_very_small_and_very_large_values(dev, cols):
         assert float((got.double() - want).abs().max()) <= 2.0 ** -11 * float(want.abs().max())
 
 
+@pytest.mark.parametrize("cols", [3, 5, 12, 20, 33])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_constant_rows_of_large_values(dev, cols, dtype):
+    """mean / sqrt(eps) is beyond fp32, xhat is 0: gx = (h - mean(h)) / sqrt(eps), lanes without columns add nothing.  h = gy: a sum of
+    cols terms, its mean, the difference and the product are off by (cols + 4) half steps of the largest term, twice."""
+    from liftreg_amd import ops_bwd
+    x = torch.full((5, cols), 2.0 ** 119, device=dev).to(dtype)
+    gy = data(dev, 5, cols, torch.float32, 12)[3].to(dtype)
+    gx, gw, gb = ops_bwd.layer_norm_bwd(x, torch.ones(cols, device=dev), torch.zeros(cols, device=dev), gy, eps=1e-6)
+    g = gy.double()
+    want = (g - g.mean(1, keepdim=True)) / float(torch.tensor(1e-6)) ** 0.5
+    half = torch.finfo(dtype).eps / 2
+    assert float((gx.double() - want).abs().max()) <= (2 * (cols + 4) * 2.0 ** -24 + half) * 2 * float(g.abs().max()) * 1e3
+    assert (gw == 0).all() and torch.isfinite(gb).all()
+
+
 @pytest.mark.parametrize("cols", [16, 801, 4097, 20_001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_that_start_anywhere(dev, cols, dtype):
