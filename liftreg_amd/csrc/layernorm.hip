@@ -21,18 +21,22 @@ constexpr int kResident = 16384;       // longest row that is held in registers:
 // arrays from this size on pass the caches by: no line of them would be there when it is read next (the last-level cache holds 256 MB; 1 GB
 // arrays forward + backward 1120 us through the caches, 1089 past them)
 constexpr int64_t kStream = (int64_t)256 << 20;
-constexpr int kBlocks = 2048;          // workgroups of the resident kernels: eight of four waves on each of 256 CUs
 
 template <class T> struct Vec;
 template <> struct Vec<float> {
   static constexpr int N = 4;
   typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+  struct Raw {             // a vector as it is fetched; four registers of their own: one that is put together from elements waits for each
+    float e[4];
+    __device__ __forceinline__ float& operator[](int i) { return e[i]; }
+  };
   static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
 };
 template <> struct Vec<uint16_t> {     // bfloat16
   static constexpr int N = 8;
   typedef uint16_t V __attribute__((ext_vector_type(8), aligned(2)));
+  typedef V Raw;
   static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
   static __device__ __forceinline__ uint16_t down(float v) {   // nearest even; NaN stays NaN
     const uint32_t u = __float_as_uint(v);
@@ -43,42 +47,68 @@ template <> struct Vec<uint16_t> {     // bfloat16
 
 // N elements from column c of a row of C (past the end: 0, not written).  A row may start at any element: gfx950 takes 16-byte
 // accesses at any address.  RAGGED = false: C is a multiple of N.  The last, partial vector of a ragged row is loaded element by
-// element or, SHIFT, as the row's last N elements, shifted down.  Measured backward, where the row's two loads feed three dependent
-// sums: bf16 (7 elements at worst) 44739 x 1500 209 us by element, 163 shifted; fp32 (3 at worst) 22362 x 3001 181 and 222.
-__device__ __forceinline__ void shifted(const uint16_t* row, int64_t c, int64_t C, float* r) {
-  typedef uint64_t Q __attribute__((ext_vector_type(2), aligned(2)));
-  const int64_t at = C - 8;
-  const Q t = *reinterpret_cast<const Q*>(row + (c < at ? c : at));
-  const int d = c < at ? 0 : (int)min(c - at, (int64_t)8);
-  const int n = 16 * (d & 3);
-  uint64_t lo = d & 4 ? t[1] : t[0], hi = d & 4 ? 0 : t[1];
-  lo = n ? lo >> n | hi << (64 - n) : lo;
-  hi >>= n;
-  if (d >= 8) lo = hi = 0;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    r[e] = Vec<uint16_t>::up((uint16_t)(lo >> (16 * e)));
-    r[e + 4] = Vec<uint16_t>::up((uint16_t)(hi >> (16 * e)));
-  }
-}
+// element, which in a wave waits for the others' whole vectors, or, SHIFT (C >= N), as the row's last N elements, which unpack()
+// shifts down: backward, where rows are fetched ahead, 30000 x 801 fp32 71 us by element and 58 shifted, 44739 x 1500 bf16 209 and 168;
+// forward the shifts cost more than they save (100000 x 801 fp32 128 and 160).  fetch() and unpack() are two steps so that rows
+// fetched ahead wait as they are: 4 registers of 8 bf16, no conversion that waits for them.
 template <bool RAGGED = true, bool SHIFT = false, bool STREAM = false, class T>
-__device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* r) {
+__device__ __forceinline__ typename Vec<T>::Raw fetch(const T* row, int64_t c, int64_t C) {
+  constexpr int N = Vec<T>::N;
+  typedef typename Vec<T>::V V;
+  typename Vec<T>::Raw r;
+  if (RAGGED && SHIFT && C >= N) {
+    const V v = *reinterpret_cast<const V*>(row + (c < C - N ? c : C - N));
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = v[e];
+  } else if (RAGGED ? c + N <= C : c < C) {
+    const V* at = reinterpret_cast<const V*>(row + c);
+    const V v = STREAM ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = v[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = RAGGED && c + e < C ? row[c + e] : (T)0;
+  }
+  return r;
+}
+template <bool RAGGED = true, bool SHIFT = false, class T = float>
+__device__ __forceinline__ void unpack(typename Vec<T>::Raw v, int64_t c, int64_t C, float* r) {
   constexpr int N = Vec<T>::N;
   if constexpr (RAGGED && SHIFT) {
     if (C >= N) {
-      shifted(row, c, C, r);
+      const int d = c < C - N ? 0 : (int)min(c - (C - N), (int64_t)N);
+      if constexpr (N == 8) {
+        typedef uint64_t Q __attribute__((ext_vector_type(2)));
+        Q t;
+        __builtin_memcpy(&t, &v, sizeof t);
+        const int n = 16 * (d & 3);
+        uint64_t lo = d & 4 ? t[1] : t[0], hi = d & 4 ? 0 : t[1];
+        lo = n ? lo >> n | hi << (64 - n) : lo;
+        hi >>= n;
+        if (d >= 8) lo = hi = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          r[e] = Vec<T>::up((uint16_t)(lo >> (16 * e)));
+          r[e + 4] = Vec<T>::up((uint16_t)(hi >> (16 * e)));
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = e < 3 && d & 1 ? v[e < 3 ? e + 1 : 3] : v[e];
+        r[3] = d & 1 ? 0.f : r[3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = d & 2 ? (e < 2 ? r[e < 2 ? e + 2 : 3] : 0.f) : r[e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = d & 4 ? 0.f : r[e];
+      }
       return;
     }
   }
-  if (RAGGED ? c + N <= C : c < C) {
-    const typename Vec<T>::V* at = reinterpret_cast<const typename Vec<T>::V*>(row + c);
-    const typename Vec<T>::V v = STREAM ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = Vec<T>::up(v[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) r[e] = RAGGED && c + e < C ? Vec<T>::up(row[c + e]) : 0.f;
-  }
+  for (int e = 0; e < N; ++e) r[e] = Vec<T>::up(v[e]);
+}
+template <bool RAGGED = true, bool STREAM = false, class T>
+__device__ __forceinline__ void load(const T* row, int64_t c, int64_t C, float* r) {
+  unpack<RAGGED, false, T>(fetch<RAGGED, false, STREAM>(row, c, C), c, C, r);
 }
 template <bool RAGGED = true, bool STREAM = false, class T>
 __device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float* r) {
@@ -234,7 +264,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
     const T* xr = x + r * C;
     float v[K * N];
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED, false, STREAM>(xr, (k * G + lane) * N, cols, v + k * N);
+    for (int k = 0; k < K; ++k) load<RAGGED, STREAM>(xr, (k * G + lane) * N, cols, v + k * N);
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
 #pragma unroll
@@ -255,27 +285,30 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 
 // gx (if set), and this workgroup's sums of g xhat and g at sw, sb (if set) + blockIdx.x * stride.  ACT: there is a LeakyReLU mask
 // (without it b is not needed: 16 of 112 registers at 16 elements a lane).  The next rows are loaded before this round's sums
-// (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.  (A workgroup of 1024
-// with several rows at a time has them all at once.)
+// (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.  (Of a workgroup of
+// 1024 with several rows at a time only fp32's: 8192 x 800 19.0 us ahead, 20.8 without; bf16 16.5 and 16.3.)
 template <class T, int G, int K, int NT, bool RAGGED, bool ACT, bool STREAM>
 __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                  const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ sw, float* __restrict__ sb,
                                                  int64_t stride, int64_t rows, int C, float inv, float eps, float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G, E = K * N;
-  constexpr bool AHEAD = E <= 8 && (NT < 1024 || G == NT);
+  constexpr bool SHIFT = N == 8 || E <= 8;      // 16 fp32 elements a lane: 1000 x 16001 66 us shifted, 52 by element
+  constexpr bool AHEAD = E <= 8 && (NT < 1024 || G == NT || N == 4);
   __shared__ float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  float wv[E], bv[ACT ? E : 1], aw[E], ab[E], v[E], g[E], nv[AHEAD ? E : 1], ng[AHEAD ? E : 1];
+  float wv[E], bv[ACT ? E : 1], aw[E], ab[E], v[E], g[E];
+  typename Vec<T>::Raw nv[K], ng[K];
   int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
-  if (AHEAD) {
-    const int cols = r < rows ? C : 0;
+  auto get = [&](int64_t at) {
+    const int cols = at < rows ? C : 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + r * C, (k * G + lane) * N, cols, (AHEAD ? nv : v) + k * N);
+    for (int k = 0; k < K; ++k) nv[k] = fetch<RAGGED, SHIFT, STREAM>(x + at * C, (k * G + lane) * N, cols);
 #pragma unroll
-    for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + r * C, (k * G + lane) * N, cols, (AHEAD ? ng : g) + k * N);
-  }
+    for (int k = 0; k < K; ++k) ng[k] = fetch<RAGGED, SHIFT, STREAM>(gy + at * C, (k * G + lane) * N, cols);
+  };
+  if (AHEAD) get(r);
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     load_f<N>(w, (k * G + lane) * N, C, 1.f, wv + k * N);
@@ -285,23 +318,13 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
   for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < rows; r0 += step, r += step) {
     const int cols = r < rows ? C : 0;
-    if (AHEAD) {
-      const int next = r + step < rows ? C : 0;
+    if (!AHEAD) get(r);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        v[i] = nv[AHEAD ? i : 0];
-        g[i] = ng[AHEAD ? i : 0];
-      }
-#pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? nv : v) + k * N);
-#pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + (r + step) * C, (k * G + lane) * N, next, (AHEAD ? ng : g) + k * N);
-    } else {
-#pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(x + r * C, (k * G + lane) * N, cols, v + k * N);
-#pragma unroll
-      for (int k = 0; k < K; ++k) load<RAGGED, sizeof(T) == 2, STREAM>(gy + r * C, (k * G + lane) * N, cols, g + k * N);
+    for (int k = 0; k < K; ++k) {
+      unpack<RAGGED, SHIFT, T>(nv[k], (k * G + lane) * N, C, v + k * N);
+      unpack<RAGGED, SHIFT, T>(ng[k], (k * G + lane) * N, C, g + k * N);
     }
+    if (AHEAD) get(r + step);
     float mean, rstd;
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
     if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
@@ -680,28 +703,40 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t size, bool backward) {
 // are not enough.  NT: lanes of a workgroup.  Backward few rows are one workgroup's, which then writes the weight's gradient itself, no
 // partial rows and no second launch: up to four rounds of 256 lanes, or of 1024 two where a row takes more than a wave (8 x 800: 7.7 us
 // in four rounds, 5.6 in one; 128 x 16: 3.2 us with 256 lanes, 3.5 with 1024).
-struct Shape { int G, E, NT; };
+// More rows, up to four rounds of 256 such workgroups, take 1024 lanes too: a quarter of the partial rows (4099 x 801 fp32 18.3 and 16.5 us,
+// bf16 17.1 and 15.2; 100000 x 800 bf16 142 and 119; with 512 lanes a row in bf16 only: 1024 x 4000 16.5 and 14.6, fp32 15.4 and 15.9).
+// `most` workgroups at once: DRAM serves a few long streams faster than many short ones, and backward each leaves a partial row of
+// 2 cols numbers.  Of 256 lanes, backward 512 in fp32 (16.8 M x 16 555 us, 671 with 2048; 100000 x 800 164 and 190), where the two
+// waves of a SIMD wait for less arithmetic than bf16's or a ragged row's, which take 1024 (16.8 M x 16 bf16 298, 339 with 512, 308
+// with 2048).  Forward 2048; fp32 of 64 MB and more 1024 (16.8 M x 16 384 and 392 us, 100000 x 800 111 and 122).
+struct Shape { int G, E, NT, most; };
 Shape shape_of(int64_t rows, int64_t cols, int vec, bool backward) {
-  Shape s = {0, 0, 256};
+  Shape s = {0, 0, 256, 2048};
   for (int G = 1; G <= 64 && !s.G; G *= 2)
     if (cols <= (int64_t)G * vec) s.G = G, s.E = vec;
   for (int G = 64; G <= 1024 && !s.G; G *= 2)
     for (int E = 8; E <= (G < 1024 ? 8 : 16) && !s.G; E *= 2)
       if (cols <= (int64_t)G * E) s.G = G, s.E = E;
   if (s.G > 256) s.NT = s.G;
-  if (backward && s.G > 64 && rows * s.G <= 2 * 1024) s.NT = 1024;
+  const int64_t lanes = rows * s.G;
+  if (backward && s.G > 64 && (lanes <= 2 * 1024 || (lanes >= 128 * 1024 && lanes <= 1024 * 1024 && s.G <= (vec == 4 ? 256 : 512)))) s.NT = 1024;
+  const bool plain = vec == 4 && cols % vec == 0;
+  if (backward) s.most = plain ? 512 : 1024;
+  else if (plain && rows * cols >= 1 << 24) s.most = 1024;
+  s.most = s.most * 256 / s.NT;
+  if (s.most < 256) s.most = 256;
   return s;
 }
 bool one_workgroup(int64_t rows, const Shape& s) { return rows * s.G <= (s.G > 64 ? 2 * 1024 : 4 * 256); }
-// Backward every workgroup leaves a partial row of 2 cols numbers: four rounds of rows each where that leaves a workgroup for every CU.
+// Backward four rounds of rows each where that leaves a workgroup for every CU.
 int64_t resident_blocks(int64_t rows, const Shape& s, bool backward) {
-  const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb, most = kBlocks * 256 / s.NT;
+  const int64_t rpb = s.NT / s.G, need = (rows + rpb - 1) / rpb;
   int64_t n = need;
   if (backward) {
     if (one_workgroup(rows, s)) return 1;
     if (n > 256) n = need / 4 > 256 ? need / 4 : 256;
   }
-  return n < most ? n : most;
+  return n < s.most ? n : s.most;
 }
 
 bool sizes_ok(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && cols <= (int64_t)1 << 31 && rows <= ((int64_t)1 << 44) / cols; }
@@ -710,8 +745,8 @@ int64_t up16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
 template <class T, int G, int K, int NT>
 void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, int64_t rows, int64_t cols, float eps, float slope,
-                hipStream_t st) {
-  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, false));
+                int64_t blocks, hipStream_t st) {
+  const dim3 grid((unsigned)blocks);
   const float inv = 1.0f / (float)cols;
 #define LR_GO(RAGGED, STREAM) \
   hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, RAGGED, STREAM>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope)
@@ -722,14 +757,13 @@ void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, 
 }
 template <class T, int G, int K, int NT>
 void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* sw, float* sb, int64_t stride, int64_t rows,
-                int64_t cols, float eps, float slope, hipStream_t st) {
-  const dim3 grid((unsigned)resident_blocks(rows, {G, K * Vec<T>::N, NT}, true));
+                int64_t cols, float eps, float slope, int64_t blocks, hipStream_t st) {
+  const dim3 grid((unsigned)blocks);
   const float inv = 1.0f / (float)cols;
 #define LR_GO(RAGGED, ACT, STREAM) \
   hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT, STREAM>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
   const bool ragged = cols % Vec<T>::N, act = slope != 1.0f, stream = rows * cols * (int64_t)sizeof(T) >= kStream;
-  if constexpr (NT == 1024 && G < NT) LR_GO(true, true, false);      // few rows: latency, which none of the three changes
-  else if (ragged && act) LR_GO(true, true, false);
+  if (ragged && act) LR_GO(true, true, false);
   else if (ragged) LR_GO(true, false, false);
   else if (act && stream) LR_GO(false, true, true);
   else if (act) LR_GO(false, true, false);
@@ -760,7 +794,7 @@ int fwd(const T* x, const float* w, const float* b, T* y, float* stats, float* w
   if (cols <= kResident) {
     constexpr int N = Vec<T>::N;
     const Shape s = shape_of(rows, cols, N, false);
-#define LR_CALL(G, K, NT) launch_fwd<T, G, K, NT>(x, w, b, y, stats, rows, cols, eps, slope, st)
+#define LR_CALL(G, K, NT) launch_fwd<T, G, K, NT>(x, w, b, y, stats, rows, cols, eps, slope, resident_blocks(rows, s, false), st)
     LR_LN_SHAPES(LR_CALL);
 #undef LR_CALL
     return lr_launch_status();
@@ -793,7 +827,7 @@ int bwd(const T* x, const float* w, const float* b, const T* gy, const float* st
     const bool part = blocks > 1 && (gw || gb);
     float *sw = part ? ws : gw, *sb = part ? ws + cols : gb;
     const int64_t stride = part ? 2 * cols : 0;
-#define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, sw, sb, stride, rows, cols, eps, slope, st)
+#define LR_CALL(G, K, NT) launch_bwd<T, G, K, NT>(x, w, b, gy, gx, sw, sb, stride, rows, cols, eps, slope, blocks, st)
     LR_LN_SHAPES(LR_CALL);
     else if (s.G == 128) LR_CALL(128, 8 / N, 1024);
     else if (s.G == 256) LR_CALL(256, 8 / N, 1024);
