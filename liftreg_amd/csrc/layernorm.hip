@@ -451,8 +451,9 @@ __device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in ever
 
 // mean and M2 of chunk blockIdx.x (`len` columns) of row blockIdx.y
 template <class T>
-__global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ x, float* __restrict__ part, int64_t C, int64_t len,
-                                                          int64_t row0) {
+__global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ x, float* __restrict__ part, int chunks, int64_t C,
+                                                          int64_t len, int64_t row0) {
+  if ((int)blockIdx.x >= chunks) return;
   constexpr int N = Vec<T>::N, K = 16 / N;
   const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
   const T* xr = x + row * C;
@@ -484,7 +485,7 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ 
   }
   p = block_join(p);
   if (threadIdx.x == 0) {
-    float* o = part + (row * gridDim.x + blockIdx.x) * 2;
+    float* o = part + (row * chunks + blockIdx.x) * 2;
     o[0] = p.mean;
     o[1] = p.m2;
   }
@@ -518,11 +519,12 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict
 template <class T>
 __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                         T* __restrict__ y, const float* __restrict__ part, float* __restrict__ stats,
-                                                        int64_t C, int64_t len, float eps, float slope, int64_t row0) {
+                                                        int chunks, int64_t C, int64_t len, float eps, float slope, int64_t row0) {
+  if ((int)blockIdx.x >= chunks) return;
   constexpr int N = Vec<T>::N;
   const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
   float mean, rstd;
-  join_stats(part, row, gridDim.x, C, len, eps, mean, rstd);
+  join_stats(part, row, chunks, C, len, eps, mean, rstd);
   if (stats && blockIdx.x == 0 && threadIdx.x == 0) {
     stats[2 * row] = mean;
     stats[2 * row + 1] = rstd;
@@ -546,7 +548,9 @@ __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x,
 template <class T, bool ACT>
 __global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                          const T* __restrict__ gy, const float* __restrict__ stats,
-                                                         float* __restrict__ part, int64_t C, int64_t len, float slope, int64_t row0) {
+                                                         float* __restrict__ part, int chunks, int64_t C, int64_t len, float slope,
+                                                         int64_t row0) {
+  if ((int)blockIdx.x >= chunks) return;
   constexpr int N = Vec<T>::N;
   __shared__ float red[4][2];
   const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
@@ -578,7 +582,7 @@ __global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x
   }
   __syncthreads();
   if (threadIdx.x < 2)
-    part[(row * gridDim.x + blockIdx.x) * 2 + threadIdx.x] =
+    part[(row * chunks + blockIdx.x) * 2 + threadIdx.x] =
         (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 
@@ -677,19 +681,25 @@ int64_t rows_at_once(int64_t rows, int64_t row_bytes) {
   return n < 32768 ? n : 32768;
 }
 
+// Chunks of 8192 columns where a row has at most 128 of them (3948 x 17000 fp32 forward 135 us, 176 with 16384, whose join reads fewer:
+// 2 x 8.4 M 46 us, 56 with 8192), of 4096 where there would be fewer than 1024 workgroups.  Where w and b (8 bytes a column) may not
+// stay in an L2 of 4 MB, a grid's row is a multiple of eight: workgroups go to the 8 XCDs in turn, and with it the same columns' w
+// and b to the same L2 (67 x 1000000 bf16 forward 73 us, 99 without; 671 x 100000, where 3 of 16 idle, 85 and 72).
 struct Plan {
   int64_t most;             // rows at a time
-  int64_t len, chunks;      // columns of a chunk (a multiple of 4096, 16384 where that makes 1024 chunks), chunks of a row (at most 1024)
+  int64_t len, chunks;      // columns of a chunk (a multiple of 4096), chunks of a row (at most 1024)
+  unsigned grid;            // workgroups of a row
   int64_t groups, span;     // row groups of the last backward pass: enough workgroups for the chip, at least 4 rows each
 };
 Plan plan_of(int64_t rows, int64_t cols, int64_t size, bool backward) {
+  auto over = [](int64_t n, int64_t d) { return (n + d - 1) / d; };
   Plan p;
   p.most = rows_at_once(rows, backward ? 0 : cols * size);
-  p.len = 16384;
-  while (p.len > 4096 && p.most * ((cols + p.len - 1) / p.len) < 1024) p.len >>= 1;
-  const int64_t least = ((cols + 1023) / 1024 + 4095) / 4096 * 4096;
-  if (p.len < least) p.len = least;
-  p.chunks = (cols + p.len - 1) / p.len;
+  p.len = over(cols, 8192) > 128 ? 16384 : 8192;
+  while (p.len > 4096 && p.most * over(cols, p.len) < 1024) p.len >>= 1;
+  if (over(cols, p.len) > 1024) p.len = over(over(cols, 1024), 4096) * 4096;
+  p.chunks = over(cols, p.len);
+  p.grid = (unsigned)(cols > 1 << 18 ? over(p.chunks, 8) * 8 : p.chunks);
   const int64_t wide = (cols + 1023) / 1024;
   p.groups = (1024 + wide - 1) / wide;
   if (p.groups > p.most / 4) p.groups = p.most / 4;
@@ -800,11 +810,12 @@ int fwd(const T* x, const float* w, const float* b, T* y, float* stats, float* w
     return lr_launch_status();
   }
   const Plan p = plan_of(rows, cols, sizeof(T), false);
-  const int64_t len = p.len, chunks = p.chunks, most = p.most;
+  const int64_t len = p.len, most = p.most;
+  const int chunks = (int)p.chunks;
   for (int64_t r = 0; r < rows; r += most) {
     const unsigned k = (unsigned)(rows - r < most ? rows - r : most);
-    hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
-    hipLaunchKernelGGL((chunk_fwd_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, y, ws, stats, cols, len, eps, slope, r);
+    hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3(p.grid, k), dim3(256), 0, st, x, ws, chunks, cols, len, r);
+    hipLaunchKernelGGL((chunk_fwd_kernel<T>), dim3(p.grid, k), dim3(256), 0, st, x, w, b, y, ws, stats, chunks, cols, len, eps, slope, r);
     const int rc = lr_launch_status();
     if (rc != LR_OK) return rc;
   }
@@ -838,9 +849,10 @@ int bwd(const T* x, const float* w, const float* b, const T* gy, const float* st
     return finish(ws, blocks, cols, gw, gb, st);
   }
   const Plan p = plan_of(rows, cols, sizeof(T), true);
-  const int64_t len = p.len, chunks = p.chunks, most = p.most, groups = p.groups, span = p.span;
+  const int64_t len = p.len, most = p.most, groups = p.groups, span = p.span;
+  const int chunks = (int)p.chunks;
   const bool inside = span * chunks <= kJoin, direct = groups == 1;
-  float* sums = ws + 2 * rows * chunks;
+  float* sums = ws + 2 * rows * p.chunks;
   float* own = sums + up16(2 * rows);
   float* part = own + up16(2 * rows);
   const dim3 grid((unsigned)((cols + 256 * Vec<T>::N - 1) / (256 * Vec<T>::N)), (unsigned)groups);
@@ -852,15 +864,15 @@ int bwd(const T* x, const float* w, const float* b, const T* gy, const float* st
     const int64_t end = r + most < rows ? r + most : rows;
     const unsigned k = (unsigned)(end - r);
     if (!stats) {
-      hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, ws, cols, len, r);
-      hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, len, eps, own, r);
+      hipLaunchKernelGGL((chunk_stats_kernel<T>), dim3(p.grid, k), dim3(256), 0, st, x, ws, chunks, cols, len, r);
+      hipLaunchKernelGGL(join_stats_kernel, dim3(k), dim3(256), 0, st, ws, chunks, cols, len, eps, own, r);
     }
-    if (act) hipLaunchKernelGGL((chunk_sums_kernel<T, true>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, sv, ws, cols, len, slope, r);
-    else hipLaunchKernelGGL((chunk_sums_kernel<T, false>), dim3((unsigned)chunks, k), dim3(256), 0, st, x, w, b, gy, sv, ws, cols, len, slope, r);
-    if (!inside) hipLaunchKernelGGL(join_sums_kernel, dim3(k), dim3(256), 0, st, ws, (int)chunks, cols, sums, r);
+    if (act) hipLaunchKernelGGL((chunk_sums_kernel<T, true>), dim3(p.grid, k), dim3(256), 0, st, x, w, b, gy, sv, ws, chunks, cols, len, slope, r);
+    else hipLaunchKernelGGL((chunk_sums_kernel<T, false>), dim3(p.grid, k), dim3(256), 0, st, x, w, b, gy, sv, ws, chunks, cols, len, slope, r);
+    if (!inside) hipLaunchKernelGGL(join_sums_kernel, dim3(k), dim3(256), 0, st, ws, chunks, cols, sums, r);
 #define LR_GO(JOIN, ACT)                                                                                                              \
   hipLaunchKernelGGL((chunk_bwd_kernel<T, JOIN, ACT>), grid, dim3(256), 0, st, x, w, b, gy, sv, inside ? ws : sums, gx, sw, sb, stride, r, \
-                     end, span, (int)chunks, cols, slope, r > 0)
+                     end, span, chunks, cols, slope, r > 0)
     if (inside && act) LR_GO(true, true);
     else if (inside) LR_GO(true, false);
     else if (act) LR_GO(false, true);
