@@ -19,7 +19,7 @@ namespace {
 
 constexpr int kResident = 16384;       // longest row that is held in registers: 1024 lanes of 16 elements
 // arrays from this size on pass the caches by: no line of them would be there when it is read next (the last-level cache holds 256 MB; 1 GB
-// arrays forward + backward 1120 us through the caches, 1089 past them)
+// arrays forward + backward 997 us through the caches, 948 past them)
 constexpr int64_t kStream = (int64_t)256 << 20;
 
 template <class T> struct Vec;
@@ -32,23 +32,25 @@ template <> struct Vec<float> {
   };
   static __device__ __forceinline__ float up(float v) { return v; }
   static __device__ __forceinline__ float down(float v) { return v; }
+  static __device__ __forceinline__ V pack(const float* r) { return V{r[0], r[1], r[2], r[3]}; }
 };
 template <> struct Vec<uint16_t> {     // bfloat16
   static constexpr int N = 8;
   typedef uint16_t V __attribute__((ext_vector_type(8), aligned(2)));
   typedef V Raw;
   static __device__ __forceinline__ float up(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
-  static __device__ __forceinline__ uint16_t down(float v) {   // nearest even; NaN stays NaN
-    const uint32_t u = __float_as_uint(v);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+  static __device__ __forceinline__ uint16_t down(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }   // nearest even
+  static __device__ __forceinline__ V pack(const float* r) {      // two in an instruction
+    typedef float F __attribute__((ext_vector_type(8)));
+    typedef __bf16 B __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(V, __builtin_convertvector((F{r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7]}), B));
   }
 };
 
 // N elements from column c of a row of C (past the end: 0, not written).  A row may start at any element: gfx950 takes 16-byte
 // accesses at any address.  RAGGED = false: C is a multiple of N.  The last, partial vector of a ragged row is loaded element by
 // element, which in a wave waits for the others' whole vectors, or, SHIFT (C >= N), as the row's last N elements, which unpack()
-// shifts down: backward, where rows are fetched ahead, 30000 x 801 fp32 71 us by element and 58 shifted, 44739 x 1500 bf16 209 and 168;
+// shifts down: backward, where rows are fetched ahead, 30000 x 801 fp32 71 us by element and 58 shifted, 44739 x 1500 bf16 209 and 155;
 // forward the shifts cost more than they save (100000 x 801 fp32 128 and 160).  fetch() and unpack() are two steps so that rows
 // fetched ahead wait as they are: 4 registers of 8 bf16, no conversion that waits for them.
 template <bool RAGGED = true, bool SHIFT = false, bool STREAM = false, class T>
@@ -114,9 +116,7 @@ template <bool RAGGED = true, bool STREAM = false, class T>
 __device__ __forceinline__ void store(T* row, int64_t c, int64_t C, const float* r) {
   constexpr int N = Vec<T>::N;
   if (c + N <= C) {
-    typename Vec<T>::V v;
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = Vec<T>::down(r[e]);
+    const typename Vec<T>::V v = Vec<T>::pack(r);
     typename Vec<T>::V* at = reinterpret_cast<typename Vec<T>::V*>(row + c);
     if (STREAM) __builtin_nontemporal_store(v, at);
     else *at = v;
@@ -672,8 +672,8 @@ __global__ __launch_bounds__(256) void chunk_bwd_kernel(const T* __restrict__ x,
 
 // ---------------------------------------------------------------- host
 // Rows of one launch: at most 32768 (a grid's y extent).  Forward also at most 144 MB of x where there is more, so that the second read
-// of a row comes from the last-level cache (256 MB): 3355 rows of 20000 fp32 columns 234 us in one go, 198 in two.  Backward, where
-// the second pass reads and writes as much again, the same made it slower (331 and 416 us): one go.
+// of a row comes from the last-level cache (256 MB): 13422 x 20000 fp32 625 us in one go, 557 in eight, bf16 420 and 354.  Backward,
+// where the second pass reads and writes as much again, it costs: 67 x 1000000 bf16 124 us in one go, 147 in two.
 int64_t rows_at_once(int64_t rows, int64_t row_bytes) {
   int64_t parts = (rows * row_bytes + ((int64_t)144 << 20) - 1) / ((int64_t)144 << 20);
   if (parts < 1) parts = 1;
@@ -712,12 +712,12 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t size, bool backward) {
 // length, and on few rows fewer loads in a row are shorter: 4099 x 801 forward 10.4 us with 16 elements, 7.5 with 8), until 1024 lanes
 // are not enough.  NT: lanes of a workgroup.  Backward few rows are one workgroup's, which then writes the weight's gradient itself, no
 // partial rows and no second launch: up to four rounds of 256 lanes, or of 1024 two where a row takes more than a wave (8 x 800: 7.7 us
-// in four rounds, 5.6 in one; 128 x 16: 3.2 us with 256 lanes, 3.5 with 1024).
+// in four rounds, 4.9 in one; 128 x 16: 3.2 us with 256 lanes, 3.5 with 1024).
 // More rows, up to four rounds of 256 such workgroups, take 1024 lanes too: a quarter of the partial rows (4099 x 801 fp32 18.3 and 16.5 us,
 // bf16 17.1 and 15.2; 100000 x 800 bf16 142 and 119; with 512 lanes a row in bf16 only: 1024 x 4000 16.5 and 14.6, fp32 15.4 and 15.9).
 // `most` workgroups at once: DRAM serves a few long streams faster than many short ones, and backward each leaves a partial row of
 // 2 cols numbers.  Of 256 lanes, backward 512 in fp32 (16.8 M x 16 555 us, 671 with 2048; 100000 x 800 164 and 190), where the two
-// waves of a SIMD wait for less arithmetic than bf16's or a ragged row's, which take 1024 (16.8 M x 16 bf16 298, 339 with 512, 308
+// waves of a SIMD wait for less arithmetic than bf16's or a ragged row's, which take 1024 (16.8 M x 16 bf16 295, 339 with 512, 308
 // with 2048).  Forward 2048; fp32 of 64 MB and more 1024 (16.8 M x 16 384 and 392 us, 100000 x 800 111 and 122).
 struct Shape { int G, E, NT, most; };
 Shape shape_of(int64_t rows, int64_t cols, int vec, bool backward) {

@@ -89,11 +89,7 @@ typedef uint32_t u1 __attribute__((aligned(1)));
 struct F32 { float x[4]; };
 
 __device__ __forceinline__ float bf_to_f(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
-__device__ __forceinline__ uint16_t f_to_bf(float f) {   // nearest even; NaN stays NaN
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+__device__ __forceinline__ uint16_t f_to_bf(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }   // nearest even
 
 // 4 elements at i of an array of n (elements past the end read as 0 and are not written).  ONCE: they are not wanted again before the
 // next step and leave the caches to the gradients, which the norm has read just before (13.5 M parameters with clipping 86 us without,
@@ -135,7 +131,9 @@ __device__ __forceinline__ void store4(float* a, int64_t i, int64_t n, const F32
 }
 __device__ __forceinline__ void store4(uint16_t* a, int64_t i, int64_t n, const F32& r) {
   if (i + 4 <= n) {
-    h4 t = {f_to_bf(r.x[0]), f_to_bf(r.x[1]), f_to_bf(r.x[2]), f_to_bf(r.x[3])};
+    typedef float F __attribute__((ext_vector_type(4)));
+    typedef __bf16 B __attribute__((ext_vector_type(4)));
+    const h4 t = __builtin_bit_cast(h4, __builtin_convertvector((F{r.x[0], r.x[1], r.x[2], r.x[3]}), B));      // two in an instruction
     __builtin_nontemporal_store(t, reinterpret_cast<h4*>(a + i));
   } else {
     for (int k = 0; k < 3; ++k)
