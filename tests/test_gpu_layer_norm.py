@@ -137,6 +137,14 @@ def test_more_long_rows_than_a_grid_has(dev):
     check(dev, *data(dev, 32770, 16_400, torch.bfloat16, 5), 1e-5, 1.0)
 
 
+@pytest.mark.parametrize("rows,cols", [(300_000, 3), (200_000, 13), (30_000, 127), (2_500, 803), (9_000, 803), (6_000, 1503), (400, 4003), (2_100, 4003),
+                                       (1_100, 8191), (600, 16_001), (60, 270_001)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("slope", [1.0, 0.2])
+def test_many_rows_that_end_inside_a_vector(dev, rows, cols, dtype, slope):
+    check(dev, *data(dev, rows, cols, dtype, rows), 1e-5, slope)
+
+
 @pytest.mark.parametrize("cols", [16, 33, 800, 4097, 20_000])
 def test_without_weight_or_bias(dev, cols):
     x, w, b, gy = data(dev, 50, cols, torch.float32, 1)
