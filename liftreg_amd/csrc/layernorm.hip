@@ -491,6 +491,18 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ 
   }
 }
 
+// f(c, end, whether the vector at c ends behind `end`) for a workgroup's vectors of [lo, hi): the whole ones four in flight, without the
+// element loads of a part, then the part
+struct Whole { static constexpr bool value = false; };
+struct Partial { static constexpr bool value = true; };
+template <int N, class F>
+__device__ __forceinline__ void whole_then_part(int64_t lo, int64_t hi, F f) {
+  int64_t c = lo + threadIdx.x * N;
+#pragma unroll 4
+  for (; c + N <= hi; c += 256 * N) f(c, c + N, Whole());
+  if (c < hi) f(c, hi, Partial());
+}
+
 // mean and rstd of a row from its chunks, by a whole workgroup
 __device__ __forceinline__ void join_stats(const float* part, int64_t row, int chunks, int64_t C, int64_t len, float eps, float& mean,
                                            float& rstd) {
@@ -529,19 +541,18 @@ __global__ __launch_bounds__(256) void chunk_fwd_kernel(const T* __restrict__ x,
     stats[2 * row] = mean;
     stats[2 * row + 1] = rstd;
   }
-#pragma unroll 4
-  for (int64_t c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
+  whole_then_part<N>(lo, hi, [&](int64_t c, int64_t end, auto part) {
     float v[N], wv[N], bv[N];
-    load(x + row * C, c, hi, v);
-    load_f<N>(w, c, hi, 1.f, wv);
-    load_f<N>(b, c, hi, 0.f, bv);
+    load<decltype(part)::value>(x + row * C, c, end, v);
+    load_f<N>(w, c, end, 1.f, wv);
+    load_f<N>(b, c, end, 0.f, bv);
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float z = fmaf((v[e] - mean) * rstd, wv[e], bv[e]);
       v[e] = z >= 0.f ? z : z * slope;
     }
-    store<true, true>(y + row * C, c, hi, v);
-  }
+    store<true, true>(y + row * C, c, end, v);
+  });
 }
 
 // sums of h and h xhat over a chunk of a row
@@ -556,24 +567,23 @@ __global__ __launch_bounds__(256) void chunk_sums_kernel(const T* __restrict__ x
   const int64_t row = row0 + blockIdx.y, lo = blockIdx.x * len, hi = min(C, lo + len);
   const float mean = stats[2 * row], rstd = stats[2 * row + 1];
   float s1 = 0.f, s2 = 0.f;
-#pragma unroll 4
-  for (int64_t c = lo + threadIdx.x * N; c < hi; c += 256 * N) {
+  whole_then_part<N>(lo, hi, [&](int64_t c, int64_t end, auto part) {
     float v[N], g[N], wv[N], bv[N];
-    load(x + row * C, c, hi, v);
-    load(gy + row * C, c, hi, g);
-    load_f<N>(w, c, hi, 1.f, wv);
-    if (ACT) load_f<N>(b, c, hi, 0.f, bv);
+    load<decltype(part)::value>(x + row * C, c, end, v);
+    load<decltype(part)::value>(gy + row * C, c, end, g);
+    load_f<N>(w, c, end, 1.f, wv);
+    if (ACT) load_f<N>(b, c, end, 0.f, bv);
     float t1 = 0.f, t2 = 0.f;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
       const float xh = (v[e] - mean) * rstd;
       const float h = (!ACT || fmaf(xh, wv[e], bv[e]) >= 0.f ? g[e] : g[e] * slope) * wv[e];
       t1 += h;
-      t2 = c + e < hi ? fmaf(h, xh, t2) : t2;
+      t2 = c + e < end ? fmaf(h, xh, t2) : t2;
     }
     s1 += t1;
     s2 += t2;
-  }
+  });
   s1 = lane_sum<64>(s1);
   s2 = lane_sum<64>(s2);
   if ((threadIdx.x & 63) == 0) {
