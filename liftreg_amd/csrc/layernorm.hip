@@ -284,7 +284,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 }
 
 // gx (if set), and this workgroup's sums of g xhat and g at sw, sb (if set) + blockIdx.x * stride.  ACT: there is a LeakyReLU mask
-// (without it b is not needed: 16 of 112 registers at 16 elements a lane).  The next rows are loaded before this round's sums
+// (without it b is not needed).  The next rows are loaded before this round's sums
 // (three dependent reductions), up to 8 elements a lane: beyond that the registers are worth more as occupancy.  (Of a workgroup of
 // 1024 with several rows at a time only fp32's: 8192 x 800 19.0 us ahead, 20.8 without; bf16 16.5 and 16.3.)
 template <class T, int G, int K, int NT, bool RAGGED, bool ACT, bool STREAM>
@@ -298,7 +298,8 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  float wv[E], bv[ACT ? E : 1], aw[E], ab[E], v[E], g[E];
+  constexpr bool HOLD = ACT && E <= 8;      // b in registers; 16 elements a lane spill then (4096 x 10000 fp32 654 us): fetched for each row (135)
+  float wv[E], bv[HOLD ? E : 1], aw[E], ab[E], v[E], g[E];
   typename Vec<T>::Raw nv[K], ng[K];
   int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
   auto get = [&](int64_t at) {
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     load_f<N>(w, (k * G + lane) * N, C, 1.f, wv + k * N);
-    if (ACT) load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + (ACT ? k * N : 0));
+    if (HOLD) load_f<N>(b, (k * G + lane) * N, C, 0.f, bv + (HOLD ? k * N : 0));
   }
 #pragma unroll
   for (int i = 0; i < E; ++i) aw[i] = ab[i] = 0.f;
@@ -329,19 +330,26 @@ __global__ __launch_bounds__(NT) void bwd_kernel(const T* __restrict__ x, const 
     row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
     if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
     float s1 = 0.f, s2 = 0.f;
+    const float* bp = b;
+    if (ACT && !HOLD) asm volatile("" : "+s"(bp));      // not out of the loop again
 #pragma unroll
-    for (int i = 0; i < E; ++i) {     // past the end g and xhat are 0 (mean rstd may be beyond fp32): nothing is added
-      const int c = (i / N * G + lane) * N + (RAGGED ? i % N : 0);
-      const float xh = (v[i] - mean) * (c < C ? rstd : 0.f);
-      float gg = g[i];
-      if (ACT) gg = fmaf(xh, wv[i], bv[ACT ? i : 0]) >= 0.f ? gg : gg * slope;
-      aw[i] = fmaf(gg, xh, aw[i]);
-      ab[i] += gg;
-      const float h = gg * wv[i];
-      s1 += h;
-      s2 = fmaf(h, xh, s2);
-      v[i] = xh;
-      g[i] = h;
+    for (int k = 0; k < K; ++k) {     // past the end g and xhat are 0 (mean rstd may be beyond fp32): nothing is added
+      float bk[N];
+      if (ACT && !HOLD) load_f<N>(bp, (k * G + lane) * N, C, 0.f, bk);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int i = k * N + e, c = (k * G + lane) * N + (RAGGED ? e : 0);
+        const float xh = (v[i] - mean) * (c < C ? rstd : 0.f);
+        float gg = g[i];
+        if (ACT) gg = fmaf(xh, wv[i], HOLD ? bv[HOLD ? i : 0] : bk[e]) >= 0.f ? gg : gg * slope;
+        aw[i] = fmaf(gg, xh, aw[i]);
+        ab[i] += gg;
+        const float h = gg * wv[i];
+        s1 += h;
+        s2 = fmaf(h, xh, s2);
+        v[i] = xh;
+        g[i] = h;
+      }
     }
     gr.sum2(s1, s2);
     if (gx) {
