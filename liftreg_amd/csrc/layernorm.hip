@@ -284,7 +284,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 }
 
 // gx (if set), and this workgroup's sums of g xhat and g at sw, sb (if set) + blockIdx.x * stride.  ACT: there is a LeakyReLU mask
-// (without it b is not needed).  The next rows are loaded before this round's sums (three dependent reductions), up to 8 elements a
+// (without it b is not needed).  The next rows are loaded before these rows' sums (three dependent reductions), up to 8 elements a
 // lane: beyond that the registers are worth more as occupancy.  (Of a workgroup of 1024 with several rows at a time only fp32's:
 // 8192 x 800 19.0 us ahead, 20.8 without; bf16 16.5 and 16.3.)  Four waves a SIMD, at most 128 registers: one ragged form took 129
 // (22362 x 3001 fp32 230 us, 170 with 128).
