@@ -10,7 +10,7 @@
 //    passes over registers.  Backward recomputes them: x is there anyway, and 8 bytes of saved statistics a row would be 1/8 of a
 //    16-channel row forward and again backward.  A lane keeps its columns over all its rows, so the weight's gradient grows in
 //    registers; groups, then waves add theirs, each workgroup leaves one partial row, a second kernel adds those in a fixed order.
-//  * longer rows are cut into chunks (few rows would leave most CUs idle): per-chunk mean and M2 (Chan's update), joined per row,
+//  * longer rows are cut into chunks (few rows would leave most CUs idle): per-chunk mean and variance (Chan's update), joined per row,
 //    then one pass that normalises; backward the same with the sums of h and h xhat, where a workgroup of the last pass owns columns
 //    and walks down the rows, so the weight's gradient needs no atomics either.
 #include "lr_common.h"
@@ -437,13 +437,15 @@ __global__ __launch_bounds__(LANES == 1 ? 256 : 1024) void finish_kernel(const f
 }
 
 // ---------------------------------------------------------------- rows that are cut into chunks
+// Chan's update.  The weight goes into the difference before the square: an empty side's mean is 0, so where one side is empty d is the
+// other's whole mean, whose square may leave fp32, and the weight 0.
 struct Part { float n, mean, m2; };
-__device__ __forceinline__ Part join(Part a, Part b) {   // Chan: exact up to rounding whatever the two sides hold
+__device__ __forceinline__ Part join(Part a, Part b) {
   Part r;
   r.n = a.n + b.n;
   const float d = b.mean - a.mean, f = r.n > 0.f ? b.n / r.n : 0.f;
   r.mean = fmaf(d, f, a.mean);
-  r.m2 = a.m2 + b.m2 + d * d * a.n * f;
+  r.m2 = fmaf(d * (a.n * f), d, a.m2 + b.m2);
   return r;
 }
 __device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in every thread
@@ -458,7 +460,7 @@ __device__ __forceinline__ Part block_join(Part p) {     // 256 threads; in ever
   return join(join(red[0], red[1]), join(red[2], red[3]));
 }
 
-// mean and M2 of chunk blockIdx.x (`len` columns) of row blockIdx.y
+// mean and variance of chunk blockIdx.x (`len` columns) of row blockIdx.y
 template <class T>
 __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ x, float* __restrict__ part, int chunks, int64_t C,
                                                           int64_t len, int64_t row0) {
@@ -496,7 +498,7 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ 
   if (threadIdx.x == 0) {
     float* o = part + (row * chunks + blockIdx.x) * 2;
     o[0] = p.mean;
-    o[1] = p.m2;
+    o[1] = p.m2 / p.n;
   }
 }
 
@@ -512,17 +514,20 @@ __device__ __forceinline__ void whole_then_part(int64_t lo, int64_t hi, F f) {
   if (c < hi) f(c, hi, Partial());
 }
 
-// mean and rstd of a row from its chunks, by a whole workgroup
+// mean and rstd of a row from its chunks, by a whole workgroup.  A chunk counts as its share of the row: the sum is then the variance and not
+// C times it, which leaves fp32 sooner.
 __device__ __forceinline__ void join_stats(const float* part, int64_t row, int chunks, int64_t C, int64_t len, float eps, float& mean,
                                            float& rstd) {
+  const float inv = 1.0f / (float)C;
   Part p = {0.f, 0.f, 0.f};
   for (int i = threadIdx.x; i < chunks; i += 256) {
     const float* o = part + (row * chunks + i) * 2;
-    p = join(p, {(float)min(len, C - i * len), o[0], o[1]});
+    const float n = (float)min(len, C - i * len) * inv;
+    p = join(p, {n, o[0], o[1] * n});
   }
   p = block_join(p);
   mean = p.mean;
-  rstd = 1.0f / sqrtf(p.m2 / (float)C + eps);
+  rstd = 1.0f / sqrtf(p.m2 / p.n + eps);
 }
 
 __global__ __launch_bounds__(256) void join_stats_kernel(const float* __restrict__ part, int chunks, int64_t C, int64_t len,

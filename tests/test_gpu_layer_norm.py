@@ -187,6 +187,42 @@ def test_constant_rows_of_large_values(dev, cols, dtype):
     assert (gw == 0).all() and torch.isfinite(gb).all()
 
 
+@pytest.mark.parametrize("cols", [16_385, 20_000, 20_001, 300_001, 1_000_000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_constant_rows_of_large_values(dev, cols, dtype):
+    """Powers of two, whose sums are exact: the mean is the value, xhat is 0 and the output the bias, however large the square of the value.
+    gx = (gy - mean(gy)) / sqrt(eps), within the bound of test_constant_rows_of_large_values with the sums' own number of half steps."""
+    from liftreg_amd import ops, ops_bwd
+    w, b = data(dev, 1, cols, torch.float32, 13)[1:3]
+    gy = data(dev, 3, cols, torch.float32, 14)[3].to(dtype)
+    eps = float(torch.tensor(1e-6))
+    for e in (56, 57, 64, 100, 119):
+        x = torch.full((3, cols), 2.0 ** e, device=dev).to(dtype)
+        y, stats = ops.layer_norm(x, w, b, eps=eps, return_stats=True)
+        assert torch.equal(y, b.to(dtype).expand(3, cols)), e
+        assert bool((stats[:, 0] == 2.0 ** e).all()) and float((stats[:, 1].double() * eps ** 0.5 - 1).abs().max()) <= 4 * U32
+        g = gy.double()
+        want = (g - g.mean(1, keepdim=True)) / eps ** 0.5
+        for s in (stats, None):
+            gx, gw, gb = ops_bwd.layer_norm_bwd(x, torch.ones_like(w), b, gy, eps=eps, stats=s)
+            half = torch.finfo(dtype).eps / 2
+            assert float((gx.double() - want).abs().max()) <= (2 * (sum_steps(cols) + 4) * U32 + half) * 2 * float(g.abs().max()) * 1e3, e
+            assert bool((gw == 0).all()) and float((gb.double() - g.sum(0)).abs().max()) <= 4 * U32 * float(g.abs().sum(0).max())
+
+
+@pytest.mark.parametrize("cols", [16_385, 20_000, 300_001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_long_rows_of_large_mean(dev, cols, dtype):
+    """Mean 2^63, spread 2^55: the square of the mean leaves fp32, those of the differences do not."""
+    x, w, b, gy = data(dev, 5, cols, torch.float32, 15, offset=300.0)
+    check(dev, (x * 2.0 ** 55).to(dtype), w, b, gy.to(dtype), 1e-5, 1.0)
+
+
+@pytest.mark.parametrize("cols", [16_385, 20_001, 300_001])
+def test_very_small_and_very_large_values_of_long_rows(dev, cols):
+    test_very_small_and_very_large_values(dev, cols)
+
+
 @pytest.mark.parametrize("cols", [16, 801, 4097, 20_001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_that_start_anywhere(dev, cols, dtype):
