@@ -160,9 +160,25 @@ __device__ __forceinline__ float add_half(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// the same of both words of an fp64 number
+__device__ __forceinline__ double words(uint32_t lo, uint32_t hi) { return __longlong_as_double((int64_t)((uint64_t)hi << 32 | lo)); }
+__device__ __forceinline__ uint32_t low(double x) { return (uint32_t)__double_as_longlong(x); }
+__device__ __forceinline__ uint32_t high(double x) { return (uint32_t)(__double_as_longlong(x) >> 32); }
+template <int CTRL>
+__device__ __forceinline__ double add_dpp(double x) {
+  return x + words((uint32_t)__builtin_amdgcn_mov_dpp((int)low(x), CTRL, 0xf, 0xf, true), (uint32_t)__builtin_amdgcn_mov_dpp((int)high(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ double add_row(double x) {
+  const auto l = __builtin_amdgcn_permlane16_swap(low(x), low(x), false, false), h = __builtin_amdgcn_permlane16_swap(high(x), high(x), false, false);
+  return words(l[0], h[0]) + words(l[1], h[1]);
+}
+__device__ __forceinline__ double add_half(double x) {
+  const auto l = __builtin_amdgcn_permlane32_swap(low(x), low(x), false, false), h = __builtin_amdgcn_permlane32_swap(high(x), high(x), false, false);
+  return words(l[0], h[0]) + words(l[1], h[1]);
+}
 // sum over aligned groups of G lanes, in every lane
-template <int G>
-__device__ __forceinline__ float lane_sum(float x) {
+template <int G, class F>
+__device__ __forceinline__ F lane_sum(F x) {
   if (G >= 2) x = add_dpp<0xB1>(x);      // neighbour
   if (G >= 4) x = add_dpp<0x4E>(x);      // pair
   if (G >= 8) x = add_dpp<0x141>(x);     // mirrored half row of 8
@@ -190,11 +206,18 @@ struct Group {
   float (*red)[2][NT / 64];
   int turn;
   __device__ __forceinline__ explicit Group(float (*r)[2][NT / 64]) : red(r), turn(0) {}
-  __device__ __forceinline__ float sum(float x) {
-    if (G <= 64) return lane_sum<G>(x);
-    float y = 0.f;
-    sum2(x, y);
-    return x;
+  __device__ __forceinline__ float sum(float x) { return across(lane_sum<(G < 64 ? G : 64)>(x)); }
+  // x: a wave's sum, in every lane.  A lane takes one wave's and lanes are added up: all of them in every lane would take W registers.
+  template <class F>
+  __device__ __forceinline__ F across(F x) {
+    if (G <= 64) return x;
+    F* buf = reinterpret_cast<F*>(red[turn]);
+    turn ^= 1;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) buf[wave] = x;
+    __syncthreads();
+    constexpr int M = W > 0 ? W : 1;
+    return lane_sum<M>(buf[wave / M * M + threadIdx.x % M]);
   }
   __device__ __forceinline__ void sum2(float& a, float& b) {
     a = lane_sum<(G < 64 ? G : 64)>(a);
@@ -218,15 +241,37 @@ struct Group {
   }
 };
 
-// mean and rstd of a row held as x[K * N]; RAGGED: cols is no multiple of N
-template <int K, int N, int G, bool RAGGED, class Gr>
-__device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int C, float inv, float eps, float& mean, float& rstd) {
-  float s = 0.f;
+// x[0] + ... + x[N-1], N a power of two, by halves: equal numbers add up without rounding
+template <int N>
+__device__ __forceinline__ float halves(const float* x) {
+  float t[N];
 #pragma unroll
-  for (int i = 0; i < K * N; ++i) s += x[i];
-  s = gr.sum(s);
-  mean = s * inv;
-  mean = fmaf(fmaf(-mean, (float)C, s), inv, mean);   // s / C rounded: a constant row has its own value as mean
+  for (int i = 0; i < N; ++i) t[i] = x[i];
+#pragma unroll
+  for (int o = N / 2; o > 0; o /= 2)
+#pragma unroll
+    for (int i = 0; i < o; ++i) t[i] += t[i + o];
+  return t[0];
+}
+// mean and rstd of a row held as x[K * N]; RAGGED: cols is no multiple of N.  A constant row has its own value as mean, which a sum in
+// fp32 misses (16384 times 1000.1: xhat 0.096 with eps = 1e-5 and not 0).  Equal numbers add up by halves without rounding: so do rows that
+// fill their lanes, and waves of longer rows that the row fills.  Elsewhere vectors are added up by halves, the rest in fp64; a row's one
+// partial vector is off by at most 2^-24 of itself, which counts where a row has few vectors: there pairs go to fp64.
+template <int K, int N, int G, bool RAGGED, class Gr>
+__device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int C, double inv, float inv32, float eps, float& mean,
+                                          float& rstd) {
+  constexpr int L = G < 64 ? G : 64, V = RAGGED && G < 16 ? 2 : N;
+  const int end = __builtin_amdgcn_readfirstlane(((K - 1) * G + (lane | (L - 1)) + 1) * N);      // of the columns that the wave can hold
+  double s;
+  if ((!RAGGED || G > 64) && end <= C) {
+    s = (double)lane_sum<L>(halves<K * N>(x) * 0x1p-10f) * 0x1p10;      // scaled: at most 1024 numbers, no further overflow
+  } else {
+    s = (double)halves<V>(x);
+#pragma unroll
+    for (int i = V; i < K * N; i += V) s += (double)halves<V>(x + i);
+    s = lane_sum<L>(s);
+  }
+  mean = (float)(gr.across(s) * inv);
   float q = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -239,17 +284,17 @@ __device__ __forceinline__ void row_stats(Gr& gr, const float* x, int lane, int 
     }
     q += RAGGED || c < C ? t : 0.f;
   }
-  const float v = fmaf(gr.sum(q), inv, eps);
+  const float v = fmaf(gr.sum(q), inv32, eps);
   rstd = v < 0x1p-100f ? __builtin_amdgcn_rsqf(v * 0x1p60f) * 0x1p30f : __builtin_amdgcn_rsqf(v);   // v_rsq_f32 takes no subnormals
 }
 
 // STREAM: x, gy, y and gx past the caches (kStream).
 template <class T, int G, int K, int NT, bool RAGGED, bool STREAM>
 __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
-                                                 T* __restrict__ y, float* __restrict__ stats, int64_t rows, int C, float inv,
-                                                 float eps, float slope) {
+                                                 T* __restrict__ y, float* __restrict__ stats, int64_t rows, int C, double inv,
+                                                 float inv32, float eps, float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G;
-  __shared__ float red[2][2][NT / 64];
+  __shared__ __attribute__((aligned(8))) float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
   float wv[K * N], bv[K * N];
@@ -266,7 +311,7 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 #pragma unroll
     for (int k = 0; k < K; ++k) load<RAGGED, STREAM>(xr, (k * G + lane) * N, cols, v + k * N);
     float mean, rstd;
-    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
+    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, inv32, eps, mean, rstd);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -291,11 +336,12 @@ __global__ __launch_bounds__(NT) void fwd_kernel(const T* __restrict__ x, const 
 template <class T, int G, int K, int NT, bool RAGGED, bool ACT, bool STREAM>
 __global__ __launch_bounds__(NT, 4) void bwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
                                                  const T* __restrict__ gy, T* __restrict__ gx, float* __restrict__ sw, float* __restrict__ sb,
-                                                 int64_t stride, int64_t rows, int C, float inv, float eps, float slope) {
+                                                 int64_t stride, int64_t rows, int C, double inv, float inv32, float eps,
+                                                 float slope) {
   constexpr int N = Vec<T>::N, RPB = NT / G, E = K * N;
   constexpr bool SHIFT = N == 8 || E <= 8;      // 16 fp32 elements a lane: 1000 x 16001 66 us shifted, 52 by element
   constexpr bool AHEAD = E <= 8 && (NT < 1024 || G == NT || N == 4);
-  __shared__ float red[2][2][NT / 64];
+  __shared__ __attribute__((aligned(8))) float red[2][2][NT / 64];
   Group<G, NT> gr(red);
   const int lane = threadIdx.x % G;
   const int64_t step = (int64_t)gridDim.x * RPB;
@@ -328,7 +374,7 @@ __global__ __launch_bounds__(NT, 4) void bwd_kernel(const T* __restrict__ x, con
     }
     if (AHEAD) get(r + step);
     float mean, rstd;
-    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, eps, mean, rstd);
+    row_stats<K, N, G, RAGGED>(gr, v, lane, C, inv, inv32, eps, mean, rstd);
     if (r >= rows) rstd = 0.f;        // no row: xhat = 0 even where eps = 0
     float s1 = 0.f, s2 = 0.f;
     const float* bp = b;
@@ -354,8 +400,8 @@ __global__ __launch_bounds__(NT, 4) void bwd_kernel(const T* __restrict__ x, con
     }
     gr.sum2(s1, s2);
     if (gx) {
-      s1 *= inv;
-      s2 *= inv;
+      s1 *= inv32;
+      s2 *= inv32;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -478,12 +524,16 @@ __global__ __launch_bounds__(256) void chunk_stats_kernel(const T* __restrict__ 
       load(xr, c, hi, v + k * N);
       have += (int)max((int64_t)0, min((int64_t)N, hi - c));
     }
-    float s = 0.f, q = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s += v[i];
+    float q = 0.f;
     Part t;
     t.n = (float)have;
-    t.mean = have ? s / t.n : 0.f;
+    t.mean = halves<16>(v) * 0.0625f;
+    if (have < 16) {         // as exact where all are equal, which halves are not
+      double s = 0.0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s += (double)v[i];
+      t.mean = have ? (float)(s / (double)have) : 0.f;
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -781,9 +831,9 @@ template <class T, int G, int K, int NT>
 void launch_fwd(const T* x, const float* w, const float* b, T* y, float* stats, int64_t rows, int64_t cols, float eps, float slope,
                 int64_t blocks, hipStream_t st) {
   const dim3 grid((unsigned)blocks);
-  const float inv = 1.0f / (float)cols;
+  const double inv = 1.0 / (double)cols;
 #define LR_GO(RAGGED, STREAM) \
-  hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, RAGGED, STREAM>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, eps, slope)
+  hipLaunchKernelGGL((fwd_kernel<T, G, K, NT, RAGGED, STREAM>), grid, dim3(NT), 0, st, x, w, b, y, stats, rows, (int)cols, inv, (float)inv, eps, slope)
   if (cols % Vec<T>::N) LR_GO(true, false);
   else if (rows * cols * (int64_t)sizeof(T) >= kStream) LR_GO(false, true);
   else LR_GO(false, false);
@@ -793,9 +843,9 @@ template <class T, int G, int K, int NT>
 void launch_bwd(const T* x, const float* w, const float* b, const T* gy, T* gx, float* sw, float* sb, int64_t stride, int64_t rows,
                 int64_t cols, float eps, float slope, int64_t blocks, hipStream_t st) {
   const dim3 grid((unsigned)blocks);
-  const float inv = 1.0f / (float)cols;
+  const double inv = 1.0 / (double)cols;
 #define LR_GO(RAGGED, ACT, STREAM) \
-  hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT, STREAM>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, eps, slope)
+  hipLaunchKernelGGL((bwd_kernel<T, G, K, NT, RAGGED, ACT, STREAM>), grid, dim3(NT), 0, st, x, w, b, gy, gx, sw, sb, stride, rows, (int)cols, inv, (float)inv, eps, slope)
   const bool ragged = cols % Vec<T>::N, act = slope != 1.0f, stream = rows * cols * (int64_t)sizeof(T) >= kStream;
   if (ragged && act) LR_GO(true, true, false);
   else if (ragged) LR_GO(true, false, false);

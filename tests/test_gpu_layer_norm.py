@@ -223,6 +223,24 @@ def test_very_small_and_very_large_values_of_long_rows(dev, cols):
     test_very_small_and_very_large_values(dev, cols)
 
 
+@pytest.mark.parametrize("cols", [1, 3, 7, 13, 33, 100, 513, 801, 1500, 4097, 5000, 10_001, 16_384, 16_385, 20_000, 20_001, 300_001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_constant_rows_of_any_value(dev, cols, dtype):
+    """The mean of a constant row is its value, also where the sum of `cols` of them is not a number of 24 bits or beyond fp32: the output is
+    the bias and the weight's gradient zero, exactly.  Without eps such a row is 0 / 0."""
+    from liftreg_amd import ops, ops_bwd
+    w, b, gy = data(dev, 6, cols, dtype, 16)[1:]
+    v = torch.tensor([1000.1, 12345.6, 0.1, -77.7, 3.3e-20, 1.1 * 2.0 ** 120], device=dev).to(dtype)
+    x = v[:, None].expand(6, cols).contiguous()
+    y, stats = ops.layer_norm(x, w, b, return_stats=True)
+    assert torch.equal(y, b.to(dtype).expand(6, cols))
+    assert stats is None or torch.equal(stats[:, 0], v.float())
+    for s in (stats, None):
+        gx, gw, gb = ops_bwd.layer_norm_bwd(x, w, b, gy, stats=s)
+        assert bool((gw == 0).all()) and bool(torch.isfinite(gx).all()) and bool(torch.isfinite(gb).all())
+    assert bool(torch.isnan(ops.layer_norm(x, w, b, eps=0.0)).all())
+
+
 @pytest.mark.parametrize("cols", [16, 801, 4097, 20_001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_that_start_anywhere(dev, cols, dtype):
