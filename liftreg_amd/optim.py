@@ -4,11 +4,15 @@ in one launch, its states in 32 bits or in block-scaled 8 bits, and the global n
 The reference trains with `torch.optim.Adam(eps=1e-5)` (src/liftreg/networks/RegistrationNet.py:245), which `AdamW` with
 `weight_decay=0` is.  GPU tensors only; launches go to torch's current stream of the tensors' device.
 """
+from collections import defaultdict
+
 import torch
 
 from . import _hip, ops
 
 BLOCK = 32                              # consecutive elements that share a scale in the 8-bit states
+_TYPES8 = {"exp_avg": torch.float8_e4m3fn, "exp_avg_scale": torch.float8_e8m0fnu, "exp_avg_sq": torch.float8_e5m2,
+           "exp_avg_sq_scale": torch.float8_e8m0fnu}
 _T = torch.Tensor
 
 
@@ -70,7 +74,7 @@ def values8(codes, scales):
 
 class AdamW(torch.optim.Optimizer):
     """AdamW on the kernel above, in torch.optim's manner: parameter groups, closures, LR schedulers, state_dict (32-bit states
-    have the keys of torch.optim.Adam / AdamW, whose checkpoints load).  `weight_decay=0` is Adam, the reference's optimizer.
+    have the keys of torch.optim.Adam / AdamW, whose checkpoints load), copies and pickles.  `weight_decay=0` is Adam, the reference's optimizer.
 
         opt = AdamW(net.parameters(), lr=1e-4, eps=1e-5, weight_decay=0.0, max_grad_norm=1.0)
 
@@ -80,6 +84,7 @@ class AdamW(torch.optim.Optimizer):
     capturable: the step count lives on the device (int64 tensor), so that `step()` can be captured in a graph; the groups'
     "lr" may then be a one-element float32 device tensor, which a replay reads.  A replay does not run Python: call the model's
     `invalidate_packed()` before inference with parameters that replays have changed.
+    These four are the constructor's: copies and pickles keep them, state_dict (groups and states) does not hold them.
     Parameters: contiguous float32 or bfloat16 GPU tensors; gradients of the parameter's type, dense."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_grad_norm=None, seed=0,
@@ -91,6 +96,19 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.max_grad_norm, self.seed, self.capturable = state_bits, max_grad_norm, int(seed), bool(capturable)
         self.grad_norm = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self):
+        # of copies and pickles; the base class keeps its own attributes only, and pickle refuses the 8-bit types
+        state = super().__getstate__() | {k: getattr(self, k) for k in ("state_bits", "max_grad_norm", "seed", "capturable", "grad_norm")}
+        if self.state_bits == 8:
+            state["state"] = {p: {k: v.view(torch.uint8) if k in _TYPES8 else v for k, v in s.items()} for p, s in self.state.items()}
+        return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self.state_bits == 8:
+            self.state = defaultdict(dict, {p: {k: v.view(_TYPES8[k]) if k in _TYPES8 and v.dtype == torch.uint8 else v for k, v in s.items()}
+                                            for p, s in self.state.items()})
 
     def add_param_group(self, group):
         b1, b2 = group.get("betas", self.defaults["betas"])
@@ -207,7 +225,7 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("amsgrad and maximize are not built")
             if group.get("weight_decay") and group.get("decoupled_weight_decay") is False:
                 raise ValueError("the checkpoint's weight_decay is an L2 term of the gradient (torch.optim.Adam), which is not built")
-        want = {"exp_avg", "exp_avg_sq"} | ({"exp_avg_scale", "exp_avg_sq_scale"} if self.state_bits == 8 else set())
+        want = set(_TYPES8) if self.state_bits == 8 else {"exp_avg", "exp_avg_sq"}
         for s in state_dict["state"].values():
             if set(s) - {"step"} != want:
                 raise ValueError(f"the checkpoint's states {sorted(s)} are not those of state_bits={self.state_bits}")

@@ -571,3 +571,21 @@ def test_gradients_in_flat_buckets(dev):
         twin(x).square().mean().backward()
         a.step(), b.step()
         assert all(torch.equal(p, q) for p, q in zip(net.parameters(), twin.parameters())), k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_copied_optimizer_takes_the_same_steps(dev, bits, capturable):
+    from liftreg_amd import optim
+    torch.manual_seed(4)
+    net = Net().to(dev)
+    opt = optim.AdamW(net.parameters(), lr=1e-2, state_bits=bits, max_grad_norm=0.1, seed=5, capturable=capturable)
+    train(net, opt, 3)
+    other, again = copy.deepcopy((net, opt))
+    train(net, opt, 2, seed=1)
+    train(other, again, 2, seed=1)
+    assert torch.equal(opt.grad_norm, again.grad_norm)
+    for p, q in zip(net.parameters(), other.parameters()):
+        assert torch.equal(p, q) and int(opt.state[p]["step"]) == int(again.state[q]["step"]) == 5
+        for k in set(opt.state[p]) - {"step"}:
+            assert torch.equal(opt.state[p][k].view(torch.uint8), again.state[q][k].view(torch.uint8))

@@ -127,3 +127,30 @@ def test_values8():
     got = values8(q, s)
     assert torch.equal(got[:32], q[:32].float()) and torch.equal(got[32:], 8 * q[32:].float())
     assert torch.isnan(values8(q, torch.tensor([255, 127], dtype=torch.uint8).view(torch.float8_e8m0fnu))[:32]).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_copies_and_pickles_of_the_optimizer(bits):
+    import copy
+    import pickle
+
+    from liftreg_amd.optim import AdamW, state8
+    p = torch.nn.Parameter(torch.ones(40))
+    opt = AdamW([p], lr=0.5, state_bits=bits, max_grad_norm=2.0, seed=(7 << 32) + 3, capturable=True)
+    count = torch.tensor(4)
+    q = torch.nn.Parameter(torch.ones(9))
+    opt.add_param_group({"params": [q], "lr": 0.25})
+    for t in (p, q):
+        m, ms, v, vs = state8(t)
+        opt.state[t] = {"step": count, "exp_avg": m, "exp_avg_sq": v, "exp_avg_scale": ms, "exp_avg_sq_scale": vs} if bits == 8 else \
+            {"step": count, "exp_avg": torch.zeros(t.shape), "exp_avg_sq": torch.ones(t.shape)}
+    opt.grad_norm = torch.tensor(1.5)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        for k in ("state_bits", "max_grad_norm", "seed", "capturable", "grad_norm"):
+            assert getattr(other, k) == getattr(opt, k), k
+        assert [g["lr"] for g in other.param_groups] == [0.5, 0.25]
+        a, b = (other.state[g["params"][0]] for g in other.param_groups)
+        assert a["step"] is b["step"] and int(a["step"]) == 4 and a["step"] is not count
+        assert a["exp_avg_sq"].dtype == (torch.float8_e5m2 if bits == 8 else torch.float32)
+        other.step()                        # no gradient: nothing to do, nothing launched
+        assert other.grad_norm is None and opt.grad_norm is not None
