@@ -9,6 +9,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include <algorithm>
+#include <deque>
 #include <string>
 #include <utility>
 #include <vector>
@@ -315,21 +316,29 @@ const at::Tensor& on_device(PyObject* o, const char* name, at::ScalarType type, 
   return t;
 }
 
-// (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, beta1, beta2, eps, weight_decay, max_norm,
-//  grad_norm, seed) -> norm or None
-PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return entry([&]() -> PyObject* {
-    arguments(n, 15);
-    const double b1 = number(a[8]), b2 = number(a[9]), eps = number(a[10]), wd = number(a[11]);
+// One AdamW step: the constructor checks the arguments and allocates, run() launches.
+// a: (params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, step, lr, beta1, beta2, eps, weight_decay, max_norm,
+//     grad_norm, seed)
+struct Step {
+  Columns c;
+  double b1, b2, eps, wd, max_norm, rate = 0.0;
+  bool eight, clip;
+  const float* rate_dev = nullptr;
+  const int64_t* step_dev = nullptr;
+  int64_t step = 1;
+  uint64_t seed;
+  at::Tensor norm, partial;
+
+  explicit Step(PyObject* const* a) : b1(number(a[8])), b2(number(a[9])), eps(number(a[10])), wd(number(a[11])) {
     if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0 && wd >= 0.0))
       fail(PyExc_ValueError, "betas must be in [0, 1), eps and weight_decay not negative; got " + std::to_string(b1) + ", " + std::to_string(b2) +
                                  ", " + std::to_string(eps) + ", " + std::to_string(wd));
-    const bool eight = a[4] != Py_None, clip = a[12] != Py_None;
+    eight = a[4] != Py_None;
+    clip = a[12] != Py_None;
     if (eight != (a[5] != Py_None)) fail(PyExc_ValueError, "8-bit states need both exp_avg_scales and exp_avg_sq_scales");
     if (!clip && a[13] != Py_None) fail(PyExc_ValueError, "grad_norm is for max_norm");
-    const double max_norm = clip ? number(a[12]) : 0.0;
+    max_norm = clip ? number(a[12]) : 0.0;
     if (clip && !(max_norm > 0.0)) fail(PyExc_ValueError, "max_norm must be positive, got " + std::to_string(max_norm));
-    Columns c;
     c.add(a[0], "params", at::kFloat, false, true);
     c.add(a[2], "exp_avgs", eight ? at::kFloat8_e4m3fn : at::kFloat, false, true);
     c.add(a[3], "exp_avg_sqs", eight ? at::kFloat8_e5m2 : at::kFloat, false, true);
@@ -339,26 +348,24 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     c.add(a[1], "grads", c.type, false, false);
     c.no_overlap();
-    const float* rate_dev = nullptr;
-    const int64_t* step_dev = nullptr;
-    double rate = 0.0;
-    int64_t step = 1;
     if (THPVariable_Check(a[7])) rate_dev = on_device(a[7], "lr", at::kFloat, c.device).data_ptr<float>();
     else rate = number(a[7]);
     if (THPVariable_Check(a[6])) step_dev = on_device(a[6], "step", at::kLong, c.device).data_ptr<int64_t>();
     else step = PyLong_AsLongLong(a[6]);
     if (step == -1 && PyErr_Occurred()) throw Set();
     if (!(rate >= 0.0) || step < 1) fail(PyExc_ValueError, "lr must not be negative and step starts at 1; got " + std::to_string(rate) + ", " + std::to_string(step));
-    const uint64_t seed = PyLong_AsUnsignedLongLongMask(a[14]);
+    seed = PyLong_AsUnsignedLongLongMask(a[14]);
     if (PyErr_Occurred()) throw Set();
     const c10::DeviceGuard guard(c.device);
-    at::Tensor norm, partial;
     if (clip && a[13] != Py_None) {
       norm = on_device(a[13], "grad_norm", at::kFloat, c.device);
     } else if (clip) {
       partial = c.partial();
       norm = empty({}, at::kFloat, c.device);
     }
+  }
+  void run() {
+    const c10::DeviceGuard guard(c.device);
     const bool own = partial.defined();
     check(lr.adamw(c.at[0].data(), c.at.back().data(), c.at[1].data(), c.at[2].data(), eight ? c.at[3].data() : nullptr,
                    eight ? c.at[4].data() : nullptr, c.numel.data(), static_cast<int>(c.n), c.type == at::kBFloat16, rate, b1, b2, eps, wd, step,
@@ -368,7 +375,31 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     // written behind autograd's back: what is kept by a parameter's version sees it
     for (const at::Tensor& t : c.keep)
       if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-    return wrap(norm);
+  }
+};
+
+// (Step's arguments) -> norm or None
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return entry([&]() -> PyObject* {
+    arguments(n, 15);
+    Step s(a);
+    s.run();
+    return wrap(s.norm);
+  });
+}
+
+// (a tuple of Step's arguments, ...) -> the last one's norm or None.  All are checked before the first is launched: a call that is refused has
+// written nothing.
+PyObject* adamw_steps(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return entry([&]() -> PyObject* {
+    std::deque<Step> steps;
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      if (!PyTuple_Check(a[i])) fail(PyExc_TypeError, "expected tuples of arguments");
+      arguments(PyTuple_GET_SIZE(a[i]), 15);
+      steps.emplace_back(&PyTuple_GET_ITEM(a[i], 0));
+    }
+    for (Step& s : steps) s.run();
+    return wrap(steps.empty() ? at::Tensor() : steps.back().norm);
   });
 }
 
@@ -395,7 +426,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(bind), METHOD(layer_norm), METHOD(layer_norm_bwd), METHOD(grad_norm), METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(bind), METHOD(layer_norm), METHOD(layer_norm_bwd), METHOD(grad_norm), METHOD(adamw_step), METHOD(adamw_steps), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of liftreg_amd.optim and ops.layer_norm (csrc/host.cpp).", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

@@ -56,6 +56,15 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         return _hip.host().adamw_step(*args)
 
 
+def _steps(calls):
+    """Several adamw_step calls (tuples of the host function's arguments), all of them checked before the first one writes."""
+    if ops._timer is None:
+        return _hip.host().adamw_steps(*calls)
+    size = sum(p.numel() * (3 * p.element_size() + (16 if c[4] is None else 4)) for c in calls for p in c[0])
+    with ops._timed("adamw_step", bytes=size):
+        return _hip.host().adamw_steps(*calls)
+
+
 def state8(p):
     """(codes e4m3, scales, codes e5m2, scales): the 8-bit states of parameter `p`, at zero."""
     def zeros(shape, dtype):
@@ -167,26 +176,30 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("max_grad_norm: all parameters must be on one device")
             norms = [grad_norm(gs) for gs in kinds.values()]
             norm = norms[0] if len(norms) == 1 else grad_norm([torch.stack(norms)])
-        eight, counted = self.state_bits == 8, set()
+        if not calls:
+            return loss
+        eight, steps = self.state_bits == 8, []
         for gi, ps, gs, ss in calls:
-            group, t = self.param_groups[gi], ss[0]["step"]
-            if isinstance(t, _T):
-                if id(t) not in counted:      # shared by several calls: counted once
-                    counted.add(id(t))
-                    t.add_(1)
-            else:
-                t += 1
-            lr = group["lr"]
-            if isinstance(lr, _T) and not lr.is_cuda:
-                lr = float(lr)
-            self.grad_norm = adamw_step(ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], step=t, lr=lr, betas=group["betas"],
-                                        eps=group["eps"], weight_decay=group["weight_decay"], max_norm=self.max_grad_norm, grad_norm=norm,
-                                        exp_avg_scales=[s["exp_avg_scale"] for s in ss] if eight else None,
-                                        exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in ss] if eight else None,
-                                        seed=self.seed + (gi << 32))      # groups draw different bits
-            if not isinstance(t, _T):
-                for s in ss:
-                    s["step"] = t
+            group, t, lr = self.param_groups[gi], ss[0]["step"], self.param_groups[gi]["lr"]
+            b1, b2 = group["betas"]
+            steps.append((ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], [s["exp_avg_scale"] for s in ss] if eight else None,
+                          [s["exp_avg_sq_scale"] for s in ss] if eight else None, t if isinstance(t, _T) else t + 1,
+                          float(lr) if isinstance(lr, _T) and not lr.is_cuda else lr, b1, b2, group["eps"], group["weight_decay"],
+                          self.max_grad_norm, norm, self.seed + (gi << 32)))      # groups draw different bits
+        # counts on the device go ahead of the launches that read them (one that several calls share once), and back if one is refused
+        ahead = list({id(s[6]): s[6] for s in steps if isinstance(s[6], _T)}.values())
+        for t in ahead:
+            t.add_(1)
+        try:
+            self.grad_norm = _steps(steps)
+        except BaseException:
+            for t in ahead:
+                t.sub_(1)
+            raise
+        for (*_, ss), s in zip(calls, steps):
+            if not isinstance(s[6], _T):
+                for state in ss:
+                    state["step"] = s[6]
         return loss
 
     def _part_counts(self, calls):

@@ -589,3 +589,49 @@ def test_a_copied_optimizer_takes_the_same_steps(dev, bits, capturable):
         assert torch.equal(p, q) and int(opt.state[p]["step"]) == int(again.state[q]["step"]) == 5
         for k in set(opt.state[p]) - {"step"}:
             assert torch.equal(opt.state[p][k].view(torch.uint8), again.state[q][k].view(torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("groups", [1, 2])
+def test_a_failed_step_with_device_counts_is_not_counted(dev, bits, groups):
+    from liftreg_amd import optim
+    net = Net().to(dev)
+    ps = [{"params": net.a.parameters()}, {"params": net.b.parameters()}] if groups == 2 else net.parameters()
+    opt = optim.AdamW(ps, capturable=True, state_bits=bits)
+    train(net, opt, 2)
+    opt.param_groups[-1]["eps"] = -1.0
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            train(net, opt, 1)
+    assert all(int(s["step"]) == 2 for s in opt.state.values())
+    opt.param_groups[-1]["eps"] = 1e-8
+    train(net, opt, 1)
+    assert all(int(s["step"]) == 3 for s in opt.state.values())
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+@pytest.mark.parametrize("clip", [None, 0.1])
+def test_a_refused_group_leaves_the_others_where_they_are(dev, capturable, clip):
+    """A step that is refused for one group or type writes nothing."""
+    from liftreg_amd import optim
+    net = Net().to(dev)
+    net.b.to(torch.bfloat16)
+    opt = optim.AdamW([{"params": [net.a.weight, net.b.weight]}, {"params": [net.a.bias, net.b.bias]}], capturable=capturable, max_grad_norm=clip)
+
+    def step(k):
+        g = torch.Generator(device="cuda").manual_seed(k)
+        for p in net.parameters():
+            p.grad = torch.randn(p.shape, device=dev, generator=g).to(p.dtype)
+        opt.step()
+
+    step(0)
+    before = [(p.detach().clone(), {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state[p].items()}) for p in net.parameters()]
+    opt.param_groups[1]["weight_decay"] = -1.0
+    with pytest.raises(ValueError):
+        step(1)
+    for p, (old, state) in zip(net.parameters(), before):
+        assert torch.equal(p, old)
+        assert all(torch.equal(v, state[k]) if isinstance(v, torch.Tensor) else v == state[k] for k, v in opt.state[p].items())
+    opt.param_groups[1]["weight_decay"] = 0.0
+    step(1)
+    assert all(not torch.equal(p, old) and int(opt.state[p]["step"]) == 2 for p, (old, _) in zip(net.parameters(), before))
