@@ -4,7 +4,7 @@ in one launch, its states in 32 bits or in block-scaled 8 bits, and the global n
 The reference trains with `torch.optim.Adam(eps=1e-5)` (src/liftreg/networks/RegistrationNet.py:245), which `AdamW` with
 `weight_decay=0` is.  GPU tensors only; launches go to torch's current stream of the tensors' device.
 """
-from collections import defaultdict
+from collections import Counter, defaultdict
 
 import torch
 
@@ -178,14 +178,15 @@ class AdamW(torch.optim.Optimizer):
             norm = norms[0] if len(norms) == 1 else grad_norm([torch.stack(norms)])
         if not calls:
             return loss
-        eight, steps = self.state_bits == 8, []
+        eight, steps, nth = self.state_bits == 8, [], Counter()
         for gi, ps, gs, ss in calls:
             group, t, lr = self.param_groups[gi], ss[0]["step"], self.param_groups[gi]["lr"]
             b1, b2 = group["betas"]
             steps.append((ps, gs, [s["exp_avg"] for s in ss], [s["exp_avg_sq"] for s in ss], [s["exp_avg_scale"] for s in ss] if eight else None,
                           [s["exp_avg_sq_scale"] for s in ss] if eight else None, t if isinstance(t, _T) else t + 1,
                           float(lr) if isinstance(lr, _T) and not lr.is_cuda else lr, b1, b2, group["eps"], group["weight_decay"],
-                          self.max_grad_norm, norm, self.seed + (gi << 32)))      # groups draw different bits
+                          self.max_grad_norm, norm, self.seed + (gi << 32) + (nth[gi] << 48)))      # groups and a group's calls draw different bits
+            nth[gi] += 1
         # counts on the device go ahead of the launches that read them (one that several calls share once), and back if one is refused
         ahead = list({id(s[6]): s[6] for s in steps if isinstance(s[6], _T)}.values())
         for t in ahead:

@@ -635,3 +635,25 @@ def test_a_refused_group_leaves_the_others_where_they_are(dev, capturable, clip)
     opt.param_groups[1]["weight_decay"] = 0.0
     step(1)
     assert all(not torch.equal(p, old) and int(opt.state[p]["step"]) == 2 for p, (old, _) in zip(net.parameters(), before))
+
+
+def test_types_of_a_group_round_with_different_bits(dev):
+    """A group with parameters of two types or two step counts is stepped in several calls, each with random bits of its own."""
+    from liftreg_amd import optim
+    n = 4096
+    start = torch.randn(n, device=dev).bfloat16()
+    ps = [torch.nn.Parameter(start.to(t)) for t in (torch.float32, torch.bfloat16)]
+    opt = optim.AdamW(ps, state_bits=8, seed=11)
+    g = (torch.randn(n, device=dev) * 1e-2).bfloat16()
+    for p in ps:
+        p.grad = g.to(p.dtype)
+    opt.step()
+    a, b = (opt.state[p] for p in ps)
+    # the same moments, the same scales, rounded apart: of 4096 codes with a remainder hundreds differ
+    assert torch.equal(a["exp_avg_scale"].view(torch.uint8), b["exp_avg_scale"].view(torch.uint8))
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert int((a[k].view(torch.uint8) != b[k].view(torch.uint8)).sum()) > 100
+    # the first call's bits are those of the seed as it is given
+    m, ms, v, vs = optim.state8(ps[0])
+    optim.adamw_step([ps[0].detach().clone()], [ps[0].grad], [m], [v], step=1, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=11)
+    assert torch.equal(a["exp_avg"].view(torch.uint8), m.view(torch.uint8)) and torch.equal(a["exp_avg_sq"].view(torch.uint8), v.view(torch.uint8))
