@@ -440,6 +440,9 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
   typedef typename State<T>::R R;
   const R b1 = (R)h.b1, b2 = (R)h.b2, c1 = (R)(1.0 - h.b1), c2 = (R)(1.0 - h.b2);
   const float eps = (float)h.eps;
+  // v_sqrt_f32 takes subnormals as 0.  Their roots, below 2^-63, are less than half a step of a larger eps; next to such a one v is scaled
+  // (always: 2.5 % more time with 8-bit states)
+  const bool tiny = __builtin_amdgcn_readfirstlane(eps < r.rbc2 * 0x1p-38f);
   R coef = 1;
   if (h.sumsq || h.norm_in) {
     R norm;
@@ -478,14 +481,24 @@ __global__ __launch_bounds__(kThreads) void adamw_kernel(T t, Hyper h) {
       for (int q = 0; q < Q; ++q) {
         const int64_t i = base + ((j + q) * kThreads + threadIdx.x) * 4;
         s[q].open();
+        float root[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const R x = (R)g[q].x[e] * coef;
           const R m = s[q].m[e] * b1 + x * c1, v = s[q].v[e] * b2 + x * x * c2;
           s[q].m[e] = m;
           s[q].v[e] = v;
-          const float den = fmaf(__builtin_amdgcn_sqrtf((float)v), r.rbc2, eps);
-          p[q].x[e] = p[q].x[e] * r.keep - r.size * ((float)m * __builtin_amdgcn_rcpf(den));
+          root[e] = __builtin_amdgcn_sqrtf((float)v);
+        }
+        if (tiny) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((float)s[q].v[e] < 0x1p-96f) root[e] = __builtin_amdgcn_sqrtf((float)s[q].v[e] * 0x1p64f) * 0x1p-32f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float den = fmaf(root[e], r.rbc2, eps);
+          p[q].x[e] = p[q].x[e] * r.keep - r.size * ((float)s[q].m[e] * __builtin_amdgcn_rcpf(den));
         }
         store4(pp, i, n, p[q]);
         s[q].store(at, i, n, r.key);

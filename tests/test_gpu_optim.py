@@ -657,3 +657,27 @@ def test_types_of_a_group_round_with_different_bits(dev):
     m, ms, v, vs = optim.state8(ps[0])
     optim.adamw_step([ps[0].detach().clone()], [ps[0].grad], [m], [v], step=1, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], seed=11)
     assert torch.equal(a["exp_avg"].view(torch.uint8), m.view(torch.uint8)) and torch.equal(a["exp_avg_sq"].view(torch.uint8), v.view(torch.uint8))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_subnormal_second_moments_without_eps(dev, bits):
+    """Gradients of 2^-50 ... 2^-69: v goes through fp32's subnormal numbers and its root does not.  The update of the first step is lr times the
+    gradient's sign within what rounding v to fp32 changes; from that v (rounded as fp32 holds it) the kernel is off by the 26 half steps of
+    test_step_with_32_bit_states."""
+    from liftreg_amd import optim
+    e = torch.arange(-50, -70, -1, device=dev, dtype=torch.float64)
+    g = (torch.exp2(e)[:, None] * torch.tensor([1.0, -1.25, 1.5, 1.75], device=dev)).reshape(-1).float()
+    lr, n = 1e-3, g.numel()
+    p = torch.zeros(n, device=dev)
+    if bits == 32:
+        m, v, more = torch.zeros(n, device=dev), torch.zeros(n, device=dev), {}
+        optim.adamw_step([p], [g], [m], [v], step=1, lr=lr, eps=0.0, weight_decay=0.0)
+        m, v = m.double(), v.double()
+    else:
+        mq, ms, vq, vs = optim.state8(p)
+        optim.adamw_step([p], [g], [mq], [vq], step=1, lr=lr, eps=0.0, weight_decay=0.0, exp_avg_scales=[ms], exp_avg_sq_scales=[vs])
+        m, v = (1 - B1) * g.double(), ((1 - B2) * g.double() ** 2).float().double()
+    assert bool((v > 0).all()) and float(v.min()) < 2.0 ** -140
+    want = -lr / (1 - B1) * m / (v.sqrt() / (1 - B2) ** 0.5)
+    assert float(((p.double() - want) / want).abs().max()) <= 26 * U32
+    assert torch.equal(torch.sign(p), -torch.sign(g))
