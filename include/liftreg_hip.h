@@ -625,7 +625,7 @@ int lr_layer_norm_bwd(const void* x, const float* w, const float* b, const void*
  *
  * lr_adamw_step: one AdamW step over n tensors, in place; 64 tensors (61 with 8-bit states) a launch:
  *     g = grad c;  m = b1 m + (1-b1) g;  v = b2 v + (1-b2) g^2
- *     p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)
+ *     p = p (1 - lr wd) - lr/(1-b1^t) m / (sqrt(v)/sqrt(1-b2^t) + eps)             (eps: 0, or at least 2^-126)
  * params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, numel: HOST arrays of n entries, read before the call
  *   returns; the entries are dev pointers to dense tensors of numel[i] elements (0 elements: the entry is skipped).  No two
  *   written tensors may overlap.  Alignment: the element's.

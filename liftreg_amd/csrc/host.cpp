@@ -330,8 +330,8 @@ struct Step {
   at::Tensor norm, partial;
 
   explicit Step(PyObject* const* a) : b1(number(a[8])), b2(number(a[9])), eps(number(a[10])), wd(number(a[11])) {
-    if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && eps >= 0.0 && wd >= 0.0))
-      fail(PyExc_ValueError, "betas must be in [0, 1), eps and weight_decay not negative; got " + std::to_string(b1) + ", " + std::to_string(b2) +
+    if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0 && (eps == 0.0 || eps >= 0x1p-126) && wd >= 0.0))
+      fail(PyExc_ValueError, "betas must be in [0, 1), eps 0 or at least 2^-126, weight_decay not negative; got " + std::to_string(b1) + ", " + std::to_string(b2) +
                                  ", " + std::to_string(eps) + ", " + std::to_string(wd));
     eight = a[4] != Py_None;
     clip = a[12] != Py_None;

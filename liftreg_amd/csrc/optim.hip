@@ -515,6 +515,9 @@ bool sizes_ok(const int64_t* numel, int n) {
   return true;
 }
 
+// v_rcp_f32 takes subnormals as 0, and where g and v are 0 the denominator is eps
+bool eps_ok(double eps) { return eps == 0.0 || eps >= 0x1p-126; }
+
 // Calls f(first, last, rounds, chunks) for each run of at most `most` tensors with elements; rounds of a chunk (see kRound): four where
 // that leaves at least `blocks` chunks of one round.
 template <class F>
@@ -618,7 +621,7 @@ extern "C" int lr_adamw_step(void* const* params, const void* const* grads, void
   if (!params || !grads || !exp_avg || !exp_avg_sq || !numel) return LR_ENULL;
   if (!exp_avg_scale != !exp_avg_sq_scale) return LR_ENULL;
   if (!sizes_ok(numel, n)) return LR_EINVAL;
-  if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0) || (!step_dev && step < 1)) return LR_EINVAL;
+  if (!(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps_ok(eps)) || (!step_dev && step < 1)) return LR_EINVAL;
   if ((norm_in || partial) && !(max_norm > 0)) return LR_EINVAL;
   if (norm_in && partial) return LR_EINVAL;
   const bool eight = exp_avg_scale != nullptr;

@@ -41,6 +41,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
     elements (`state8` makes them, `values8` reads them).  They are rounded stochastically: the random bits are a function of
     (seed, step, position of the element in the call's tensors), so equal calls give equal bits.  A block with an element that is
     not finite becomes NaN as a whole.
+    eps: 0 or at least 2^-126 (it is added in fp32).  With 0 a v below 2^-149, which fp32 holds as 0, divides by 0.
     step: 1 for the first step; lr: both numbers, or one-element device tensors (int64, float32) that a captured graph reads
     at each replay (a number is captured as it is).
     max_norm: the gradients are scaled by min(1, max_norm / (norm + 1e-6)) on the way in (they are not written); norm is
@@ -122,9 +123,10 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         b1, b2 = group.get("betas", self.defaults["betas"])
         lr = group.get("lr", self.defaults["lr"])
-        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not lr >= 0.0 or group.get("eps", self.defaults["eps"]) < 0.0 or \
+        eps = group.get("eps", self.defaults["eps"])
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0) or not lr >= 0.0 or not (eps == 0.0 or eps >= 2.0 ** -126) or \
                 group.get("weight_decay", self.defaults["weight_decay"]) < 0.0:
-            raise ValueError("betas must be in [0, 1), lr, eps and weight_decay not negative")
+            raise ValueError("betas must be in [0, 1), eps 0 or at least 2^-126, lr and weight_decay not negative")
         if isinstance(lr, _T) and lr.is_cuda and not self.capturable:
             raise ValueError("a learning rate on the device needs capturable=True")
         super().add_param_group(group)

@@ -154,3 +154,20 @@ def test_copies_and_pickles_of_the_optimizer(bits):
         assert a["exp_avg_sq"].dtype == (torch.float8_e5m2 if bits == 8 else torch.float32)
         other.step()                        # no gradient: nothing to do, nothing launched
         assert other.grad_norm is None and opt.grad_norm is not None
+
+
+def test_an_eps_that_fp32_holds_with_fewer_bits_is_refused(hip):
+    """eps is added in fp32: 0, or a normal number."""
+    from liftreg_amd import optim
+    f = C.addressof(C.c_float(0))
+    n, ptr = np.array([5], dtype=np.int64), np.array([f], dtype=np.uint64)
+    at = lambda a: a.ctypes.data
+    x = torch.zeros(3)
+    for eps in (1e-40, 5e-324, 2.0 ** -127):
+        assert hip.lib().lr_adamw_step(at(ptr), at(ptr), at(ptr), at(ptr), None, None, at(n), 1, 0, 1e-3, 0.9, 0.999, eps, 0.0, 1, None, None, 0.0,
+                                       None, None, None, 0, None) == -1
+        with pytest.raises(ValueError):
+            optim.adamw_step([x], [x], [x], [x], step=1, eps=eps)
+        with pytest.raises(ValueError):
+            optim.AdamW([torch.nn.Parameter(x)], eps=eps)
+    optim.AdamW([torch.nn.Parameter(x)], eps=2.0 ** -126), optim.AdamW([torch.nn.Parameter(x)], eps=0.0)
