@@ -241,6 +241,15 @@ def test_constant_rows_of_any_value(dev, cols, dtype):
     assert bool(torch.isnan(ops.layer_norm(x, w, b, eps=0.0)).all())
 
 
+@pytest.mark.parametrize("cols", [16, 800, 8192])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("slope", [1.0, 0.2])
+def test_arrays_that_pass_the_caches_by(dev, cols, dtype, slope):
+    """From 256 MiB on x, gy, y and gx are read and written past the caches."""
+    rows = (256 << 20) // (cols * torch.finfo(dtype).bits // 8) + 3
+    check(dev, *data(dev, rows, cols, dtype, 18), 1e-5, slope)
+
+
 @pytest.mark.parametrize("cols", [16, 801, 4097, 20_001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_views_that_start_anywhere(dev, cols, dtype):

@@ -681,3 +681,66 @@ def test_subnormal_second_moments_without_eps(dev, bits):
     want = -lr / (1 - B1) * m / (v.sqrt() / (1 - B2) ** 0.5)
     assert float(((p.double() - want) / want).abs().max()) <= 26 * U32
     assert torch.equal(torch.sign(p), -torch.sign(g))
+
+
+# above 2048 x 1024 elements a launch takes chunks of 4096, above 2048 x 4096 a workgroup takes several of them
+LARGE = [[3, 1_000_003, 5000, 4097, 970_001, 1, 200_000], [5_000_001, 33, 3_400_003, 12_289, 7]]
+
+
+@pytest.mark.parametrize("sizes", LARGE, ids=lambda s: f"{len(s)}x{sum(s)}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("clip", [None, 0.5])
+def test_large_steps_with_32_bit_states(dev, sizes, dtype, clip):
+    assert 2048 * 1024 < sum(sizes) < 2048 * 4096 or sum(sizes) > 2048 * 4096
+    test_step_with_32_bit_states(dev, sizes, dtype, True, clip)
+
+
+def step_with_8_bit_states(dev, sizes, dtype, steps, clip):
+    """test_step_with_8_bit_states with clipping, a step at a time (the moments of a step are formed from the codes that the last one left)."""
+    from liftreg_amd import optim
+    p, g = tensors(dev, sizes, dtype, 17)
+    st = [optim.state8(t) for t in p]
+    (m, ms, v, vs), seed = map(list, zip(*st)), (3 << 32) + 12345
+    host = lambda ts: [t.double().cpu().numpy() for t in ts]
+    grads = host(g)
+    want_norm = float(np.sqrt(sum((x ** 2).sum() for x in grads)))
+    for step in range(1, steps + 1):
+        old = [host(p), grads, host([optim.values8(a, b) for a, b in zip(m, ms)]), host([optim.values8(a, b) for a, b in zip(v, vs)])]
+        norm = optim.adamw_step(p, g, m, v, step=step, lr=1e-3, weight_decay=0.1, max_norm=clip, exp_avg_scales=ms, exp_avg_sq_scales=vs, seed=seed)
+        assert (norm is None) == (clip is None) and (clip is None or abs(float(norm) - want_norm) <= 2 * U32 * want_norm)
+        coef = 1.0 if clip is None else min(1.0, clip / (want_norm + 1e-6))
+        assert clip is None or coef < 0.5
+        first = 0
+        for i, n in enumerate(sizes):
+            wp, wm, wv, upd = definition(*(o[i] for o in old), step, 1e-3, 1e-8, 0.1, clip, want_norm)
+            rm, rv = random16(seed, step, first, n)
+            first += -(-n // 32) * 32
+            for q, s, want, r, top, man, least in ((m[i], ms[i], wm, rm, 7, 3, 2.0 ** -9), (v[i], vs[i], wv, rv, 14, 2, 2.0 ** -16)):
+                y, low, grid = neighbours8(want, top, man, least, s.view(torch.uint8).cpu().numpy().astype(int) - 127)
+                got = q.to(torch.float32).double().cpu().numpy()
+                frac = (y - low) / grid
+                # moments in fp64: what is off is the coefficient, by a few 2^-53 of terms no larger than 2^17 grid steps
+                sure = np.abs(frac + r - 1) > 2.0 ** -30
+                assert sure.mean() > 0.99 or n < 100
+                pick = np.where(frac + r >= 1, low + grid, low)
+                if top == 14:
+                    pick = np.where((want > 0) & (pick == 0), least, pick)
+                assert np.array_equal(np.abs(got)[sure], pick[sure])
+                assert (np.sign(got)[got != 0] == np.sign(want)[got != 0]).all()
+            size = 1e-3 / (1 - B1 ** step) / (np.sqrt(wv) / np.sqrt(1 - B2 ** step) + 1e-8)
+            tol_m = 8 * U32 * (np.abs(B1 * old[2][i]) + np.abs((1 - B1) * coef * grads[i]))
+            tol = 26 * U32 * np.abs(upd) + size * tol_m + 3 * U32 * np.abs(wp) + (UBF * np.abs(wp) if dtype == torch.bfloat16 else 0)
+            assert (np.abs(p[i].double().cpu().numpy() - wp) <= tol + 1e-44).all()
+
+
+@pytest.mark.parametrize("sizes", LARGE, ids=lambda s: f"{len(s)}x{sum(s)}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("clip", [None, 0.5])
+def test_large_steps_with_8_bit_states(dev, sizes, dtype, clip):
+    step_with_8_bit_states(dev, sizes, dtype, 1, clip)
+
+
+@pytest.mark.parametrize("sizes", [[31, 32, 33], [7, 4096, 4097], [5, 27 * 48, 3, 8191, 70001], [13] * 130], ids=lambda s: f"{len(s)}x{sum(s)}")
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clipped_steps_with_8_bit_states(dev, sizes, dtype):
+    step_with_8_bit_states(dev, sizes, dtype, 3, 1e-3)
