@@ -171,6 +171,10 @@ def host():
             from . import _host as module
         except ImportError as e:
             raise LiftRegHipError(f"liftreg_amd/_host.so cannot be loaded ({e}): build it with `make -C liftreg_amd/csrc`") from e
+        built = getattr(module, "torch_version", "of unknown version")
+        if built != torch.__version__:
+            raise LiftRegHipError(f"liftreg_amd/_host.so was compiled against torch {built}, this is {torch.__version__}: "
+                                  "build it again with `make -C liftreg_amd/csrc`")
         module.bind(LiftRegHipError, torch._C._cuda_getCurrentRawStream,
                     *(C.cast(getattr(handle, n), C.c_void_p).value for n in (
                         "lr_strerror", "lr_layer_norm_resident_cols", "lr_layer_norm_workspace", "lr_layer_norm", "lr_layer_norm_bwd",

@@ -432,4 +432,14 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host side of liftreg_amd.
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host() { return PyModule_Create(&module); }
+#define TEXT_OF(x) #x
+#define TEXT(x) TEXT_OF(x)
+
+PyMODINIT_FUNC PyInit__host() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TEXT(LR_TORCH)) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -171,3 +171,14 @@ def test_an_eps_that_fp32_holds_with_fewer_bits_is_refused(hip):
         with pytest.raises(ValueError):
             optim.AdamW([torch.nn.Parameter(x)], eps=eps)
     optim.AdamW([torch.nn.Parameter(x)], eps=2.0 ** -126), optim.AdamW([torch.nn.Parameter(x)], eps=0.0)
+
+
+def test_the_host_module_belongs_to_the_torch_that_is_loaded(hip, monkeypatch):
+    """_host.so is compiled against torch's C++ headers: under another torch it is refused, not called."""
+    assert hip.host().torch_version == torch.__version__
+    monkeypatch.setattr(hip, "_host", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.0+other")
+    with pytest.raises(hip.LiftRegHipError, match="0.0.0"):
+        hip.host()
+    monkeypatch.undo()
+    assert hip.host().torch_version == torch.__version__
