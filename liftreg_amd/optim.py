@@ -243,16 +243,17 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the checkpoint's weight_decay is an L2 term of the gradient (torch.optim.Adam), which is not built")
         want = set(_TYPES8) if self.state_bits == 8 else {"exp_avg", "exp_avg_sq"}
         for s in state_dict["state"].values():
-            if set(s) - {"step"} != want:
+            if set(s) != want | {"step"}:
                 raise ValueError(f"the checkpoint's states {sorted(s)} are not those of state_bits={self.state_bits}")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         ours = [p for g in self.param_groups for p in g["params"]]
         held = [(p, state_dict["state"][i]) for i, p in zip(ids, ours) if i in state_dict["state"]]
-        like = {8: (torch.float8_e4m3fn, torch.float8_e5m2), 32: (torch.float32, torch.float32)}[self.state_bits]
         for p, src in held:
-            for k, dtype in zip(("exp_avg", "exp_avg_sq"), like):
-                if tuple(src[k].shape) != tuple(p.shape) or src[k].dtype != dtype:
-                    raise ValueError(f"the checkpoint's {k} is {src[k].dtype} {tuple(src[k].shape)}, needed: {dtype} {tuple(p.shape)}")
+            for k in sorted(want):
+                dtype = _TYPES8[k] if self.state_bits == 8 else torch.float32
+                shape = (-(-p.numel() // BLOCK),) if k.endswith("_scale") else tuple(p.shape)
+                if tuple(src[k].shape) != shape or src[k].dtype != dtype:
+                    raise ValueError(f"the checkpoint's {k} is {src[k].dtype} {tuple(src[k].shape)}, needed: {dtype} {shape}")
         super().load_state_dict(state_dict)
         # the base class casts every state to its parameter's type: take the checkpoint's own values again
         shared = {}

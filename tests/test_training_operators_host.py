@@ -182,3 +182,23 @@ def test_the_host_module_belongs_to_the_torch_that_is_loaded(hip, monkeypatch):
         hip.host()
     monkeypatch.undo()
     assert hip.host().torch_version == torch.__version__
+
+
+def test_load_state_dict_refuses_states_before_it_changes_anything():
+    from liftreg_amd.optim import AdamW, state8
+    p = [torch.nn.Parameter(torch.ones(40))]
+
+    def checkpoint(**more):
+        opt = AdamW(p, lr=0.5, state_bits=8)
+        m, ms, v, vs = state8(p[0])
+        opt.state[p[0]] = {"step": 3, "exp_avg": m, "exp_avg_scale": ms, "exp_avg_sq": v, "exp_avg_sq_scale": vs} | more
+        return opt.state_dict()
+
+    without = checkpoint()
+    del without["state"][0]["step"]
+    scales = torch.zeros(3, dtype=torch.uint8)
+    for bad in (without, checkpoint(exp_avg_scale=scales.view(torch.float8_e8m0fnu)), checkpoint(exp_avg_sq_scale=scales[:2])):
+        opt = AdamW(p, lr=0.25, state_bits=8)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(bad)
+        assert opt.param_groups[0]["lr"] == 0.25 and not opt.state
