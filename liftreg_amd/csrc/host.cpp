@@ -155,7 +155,8 @@ Norm norm_arguments(PyObject* x, PyObject* w, PyObject* b, PyObject* eps, PyObje
   if (n.x.dim() < 1 || n.x.size(-1) < 1) fail(PyExc_ValueError, "x must have a last axis to normalise, got shape " + shape_of(n.x));
   n.eps = number(eps);
   n.slope = number(slope);
-  if (!(n.eps >= 0.0)) fail(PyExc_ValueError, "eps must not be negative, got " + std::to_string(n.eps));
+  if (!(n.eps >= 0.0) || (n.eps > 0.0 && static_cast<float>(n.eps) == 0.f))
+    fail(PyExc_ValueError, "eps must be 0 or a positive fp32 number");
   on_gpu(n.x, "x");
   n.x = n.x.contiguous();
   n.w = norm_param(w, "weight", n.x);

@@ -792,7 +792,9 @@ def linear_lrelu(x, weight, bias, negative_slope=1.0):
 # ----------------------------------------------------------------------------- layer norm
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5, negative_slope=1.0, return_stats=False):
     """LeakyReLU(layer norm of x over its last axis * weight + bias), one pass (negative_slope = 1: no activation).
-    x: (..., C) float32 or bfloat16, any number of rows; weight, bias: (C,) float32 or None; y in x's type, statistics in float32.
+    eps: 0 (a constant row is then 0 / 0) or a positive fp32 number.
+    x: (..., C) float32 or bfloat16, any number of rows; weight, bias: (C,) float32 or None; y in x's type, statistics in float32
+    (values up to 2^123, differences from their row's mean up to 2^53: squares are summed in fp32).
     return_stats: (y, stats) for ops_bwd.layer_norm_bwd: a (rows, 2) tensor of mean and 1 / sqrt(var + eps), or None for rows of
     at most lr_layer_norm_resident_cols() columns, whose backward pass recomputes them from the row it holds in registers."""
     if _timer is None:

@@ -202,3 +202,17 @@ def test_load_state_dict_refuses_states_before_it_changes_anything():
         with pytest.raises(ValueError):
             opt.load_state_dict(bad)
         assert opt.param_groups[0]["lr"] == 0.25 and not opt.state
+
+
+def test_a_layer_norm_eps_that_fp32_rounds_to_zero_is_refused(hip):
+    """It would divide a constant row's 0 by 0."""
+    from liftreg_amd import ops, ops_bwd
+    x = torch.zeros(3, 4)
+    for eps in (1e-46, 1e-300):
+        with pytest.raises(ValueError):
+            ops.layer_norm(x, eps=eps)
+        with pytest.raises(ValueError):
+            ops_bwd.layer_norm_bwd(x, None, None, x, eps=eps)
+    for eps in (0.0, 1e-44):
+        with pytest.raises(hip.LiftRegHipError):         # next in line: a tensor on the CPU
+            ops.layer_norm(x, eps=eps)
