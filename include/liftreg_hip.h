@@ -608,7 +608,8 @@ int lr_jacobi_det_stats_f32(const float* map, int B, int D, int W, int H, float 
  *     g = gy (z >= 0 ? 1 : slope),  h = g w,  gx = (h - mean(h) - xhat mean(h xhat)) / sqrt(var + eps)
  *     gw = sum over rows of g xhat,  gb = sum over rows of g
  * x, y, gy, gx: dev, fp32 or (bf16 != 0) bfloat16, any alignment of their elements; w, b (cols): dev fp32, nullable (1 and 0);
- * gx, gw, gb nullable (not computed).  Sums in fp32, fixed order.  rows >= 0, cols >= 1.
+ * gx, gw, gb nullable (not computed).  Sums in fp32, fixed order; a constant row has its own value as mean.  Values up to 2^123,
+ * differences from their row's mean up to 2^53.  eps >= 0 (0: a constant row is 0 / 0).  rows >= 0, cols >= 1.
  * stats: dev fp32 (rows, 2), mean and 1 / sqrt(var + eps).  lr_layer_norm writes it if it is not NULL.  lr_layer_norm_bwd reads
  *   it if it is not NULL (and rows are longer than lr_layer_norm_resident_cols(): shorter ones are held in registers, where
  *   recomputing the statistics costs less than reading them).

@@ -1,5 +1,5 @@
-// optim.hip — the update of the network's parameters: the AdamW step over all the tensors of a model in one launch (64 tensors a
-// launch), with 32-bit or block-scaled 8-bit states, and the global norm of the gradients it clips by.
+// optim.hip — the update of the network's parameters: the AdamW step over all the tensors of a model (64 tensors a launch, 61 with
+// 8-bit states), with 32-bit or block-scaled 8-bit states, and the global norm of the gradients it clips by.
 //
 // The reference trains with torch.optim.Adam (src/liftreg/networks/RegistrationNet.py:245); with weight_decay = 0 this is its step.
 //   g = grad * c,  c = min(1, max_norm / (|grad|_2 + 1e-6))         (c = 1 without clipping)

@@ -1,5 +1,5 @@
-"""The update of the parameters on the HIP kernels (liftreg_amd/csrc/optim.hip): the AdamW step over all the tensors of a model
-in one launch, its states in 32 bits or in block-scaled 8 bits, and the global norm of the gradients that it clips by.
+"""The update of the parameters on the HIP kernels (liftreg_amd/csrc/optim.hip): the AdamW step over all the tensors of a model,
+64 of them a launch, its states in 32 bits or in block-scaled 8 bits, and the global norm of the gradients that it clips by.
 
 The reference trains with `torch.optim.Adam(eps=1e-5)` (src/liftreg/networks/RegistrationNet.py:245), which `AdamW` with
 `weight_decay=0` is.  GPU tensors only; launches go to torch's current stream of the tensors' device.
@@ -93,7 +93,8 @@ class AdamW(torch.optim.Optimizer):
     seed: of the stochastic rounding of 8-bit states.
     capturable: the step count lives on the device (int64 tensor), so that `step()` can be captured in a graph; the groups'
     "lr" may then be a one-element float32 device tensor, which a replay reads.  A replay does not run Python: call the model's
-    `invalidate_packed()` before inference with parameters that replays have changed.
+    `invalidate_packed()` before inference with parameters that replays have changed.  A graph keeps the state tensors and counts of its
+    capture: load checkpoints before it, and step the same parameters between replays (others would part from a shared count).
     These four are the constructor's: copies and pickles keep them, state_dict (groups and states) does not hold them.
     Parameters: contiguous float32 or bfloat16 GPU tensors; gradients of the parameter's type, dense."""
 
